@@ -60,6 +60,34 @@ class TensorInfo(C.Structure):
                 ("dtype", C.c_char * 16)]
 
 
+class PagedKv(C.Structure):
+    """bybycu_paged_kv: one layer's paged cache and the batch of a call."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("page_stride", C.c_int64), ("head_stride", C.c_int64),
+                ("token_stride", C.c_int64), ("page_table", C.c_void_p), ("table_stride", C.c_int64),
+                ("q_start", C.c_void_p), ("kv_lens", C.c_void_p), ("n_pages", C.c_int32), ("page_size", C.c_int32),
+                ("kv_heads", C.c_int32), ("head_dim", C.c_int32), ("max_pages", C.c_int32), ("n_seqs", C.c_int32),
+                ("n_tokens", C.c_int32), ("reserved", C.c_int32)]
+
+
+class Rope(C.Structure):
+    """bybycu_rope: the arguments of bybycu_rope_append."""
+    _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("q_out", C.c_void_p),
+                ("q_token_stride", C.c_int64), ("q_head_stride", C.c_int64), ("k_token_stride", C.c_int64),
+                ("k_head_stride", C.c_int64), ("v_token_stride", C.c_int64), ("v_head_stride", C.c_int64),
+                ("out_token_stride", C.c_int64), ("out_head_stride", C.c_int64), ("turns", C.c_void_p),
+                ("positions", C.c_void_p), ("in_dtype", C.c_int32), ("q_heads", C.c_int32), ("pairs", C.c_int32),
+                ("interleaved", C.c_int32), ("magnitude", C.c_float), ("reserved", C.c_int32)]
+
+
+class Attention(C.Structure):
+    """bybycu_attention: the arguments of bybycu_paged_attention."""
+    _fields_ = [("q", C.c_void_p), ("out", C.c_void_p), ("q_token_stride", C.c_int64), ("q_head_stride", C.c_int64),
+                ("out_token_stride", C.c_int64), ("out_head_stride", C.c_int64), ("slopes", C.c_void_p),
+                ("prefix_lens", C.c_void_p), ("out_dtype", C.c_int32), ("q_heads", C.c_int32), ("max_q", C.c_int32),
+                ("max_kv", C.c_int32), ("window", C.c_int32), ("route", C.c_int32), ("scale", C.c_float),
+                ("softcap", C.c_float)]
+
+
 class BybyCudaError(RuntimeError):
     def __init__(self, code: int, message: str):
         super().__init__(f"[cuda] {message} (status {code})")
@@ -98,6 +126,10 @@ SIGNATURES = {
                                C.POINTER(_vp), _vp, _vp, C.c_float, _i32, _i32, _i32, _vp],
     "bybycu_session_matmul_q4_fused": [_i32, _vp, _i32, C.POINTER(_vp), C.POINTER(_vp), C.POINTER(_vp),
                                        C.POINTER(_i32), C.POINTER(_vp), _vp, _vp, C.c_float, _i32, _i32, _i32],
+    "bybycu_rope_append": [C.POINTER(PagedKv), C.POINTER(Rope), _vp],
+    "bybycu_paged_attention": [C.POINTER(PagedKv), C.POINTER(Attention), _vp],
+    "bybycu_copy_pages": [_vp, _vp, _i32, _i64, _i64, _i64, _i32, _vp, _i32, _vp],
+    "bybycu_beam_select": [_vp, _i32, _i64, _vp, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp],
     "bybycu_session_begin": [],
     "bybycu_session_end": [],
     "bybycu_session_upload": [_vp, _i64, C.POINTER(_vp)],

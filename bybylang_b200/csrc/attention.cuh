@@ -1,0 +1,81 @@
+// attention.cuh - what the paged-attention kernels share: their parameters, which keys a row
+// sees, and the score of a pair.
+#pragma once
+
+#include "kvcache.cuh"
+
+namespace bybycu {
+namespace attn {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct Params {
+    const __nv_bfloat16* q;
+    void* out;
+    int64_t q_token, q_head, o_token, o_head;
+    const float* slopes;
+    const int32_t* prefix;
+    int32_t q_heads, group, max_q, max_kv, window;   // group: query heads a kv head
+    float scale_log2, cap, scale_over_cap;           // scale * log2(e); softcap; scale / softcap
+};
+
+// One sequence of the batch as a kernel reads it.  rows and kv are what may be touched: never past
+// the tensors, the table or what the launch was sized for; a sequence that is longer keeps its
+// positions, loses the rest and is recorded.
+struct Seq {
+    int q0, rows, kv, first_pos, prefix;
+};
+
+__device__ __forceinline__ Seq load_seq(const kvc::Cache& c, const Params& p, int b) {
+    Seq s;
+    s.q0 = c.q_start[b];
+    const int nq = c.q_start[b + 1] - s.q0, kv = c.kv_lens[b], limit = min(p.max_kv, c.max_pages * c.page_size);
+    s.prefix = p.prefix ? p.prefix[b] : 0;
+    s.first_pos = kv - nq;
+    s.rows = min(nq, p.max_q);
+    if (s.q0 < 0 || s.q0 > c.n_tokens) s.rows = 0;
+    else s.rows = min(s.rows, c.n_tokens - s.q0);
+    s.kv = min(kv, limit);
+    if ((s.rows != nq || s.kv != kv) && (threadIdx.x & 31) == 0) record_device_error(kDevErrLength);
+    return s;
+}
+
+// Keys [lo, hi) that a row at position pos can see: j <= pos or j < prefix, within the cache and
+// the window.  Empty (lo >= hi) for a padding row.
+__device__ __forceinline__ void row_range(const Params& p, const Seq& s, int pos, int* lo, int* hi) {
+    *hi = pos < 0 ? 0 : min(s.kv, max(pos + 1, s.prefix));
+    *lo = p.window > 0 ? max(0, pos - p.window + 1) : 0;
+}
+
+// The score of a pair in units of log2: raw = q . k.
+//   MOD: a tanh cap and / or distance slopes.  tanh(y) = 1 - 2 / (1 + e^2y) with the hardware's
+//   exponential and reciprocal: its absolute error is a few 2^-24, times the cap.
+template <bool MOD>
+__device__ __forceinline__ float score_log2(const Params& p, float raw, float slope_log2, int distance) {
+    if constexpr (!MOD) {
+        return raw * p.scale_log2;
+    } else {
+        float s;
+        if (p.cap > 0.0f) {
+            const float y = raw * p.scale_over_cap;
+            s = p.cap * kLog2e * (1.0f - __fdividef(2.0f, 1.0f + exp2f(2.0f * kLog2e * y)));
+        } else {
+            s = raw * p.scale_log2;
+        }
+        return s - slope_log2 * static_cast<float>(distance < 0 ? -distance : distance);
+    }
+}
+
+// Where the token at position j of sequence b is, or -1 (recorded) for a page that does not exist.
+__device__ __forceinline__ int64_t slot_of(const kvc::Cache& c, int b, int j) {
+    const int pg = j / c.page_size;
+    const int id = c.page_table[b * c.table_stride + pg];
+    if (id < 0 || id >= c.n_pages) {
+        record_device_error(kDevErrPage);
+        return -1;
+    }
+    return id * c.page_stride + (j - pg * c.page_size) * c.token_stride;
+}
+
+}  // namespace attn
+}  // namespace bybycu

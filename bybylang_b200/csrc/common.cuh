@@ -49,6 +49,8 @@ enum DeviceErr : uint32_t {
     kDevErrTmemAlloc = 6,   // tensor memory allocation failed
     kDevErrActRange = 7,    // an activation has no image in the route's operand format (out of range, inf, NaN)
     kDevErrSplitWait = 8,   // a split-K part's partial sums never arrived
+    kDevErrPage = 9,        // a page id or a position outside the paged cache
+    kDevErrLength = 10,     // a sequence longer than the call's max_q or max_kv
 };
 
 __device__ uint32_t g_device_error = 0;

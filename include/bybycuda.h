@@ -325,6 +325,99 @@ BYBYCU_API int bybycu_tuning_stats(int* prepared_plans, int64_t* tuned_dispatche
 /* The plan cache file of the current device ("" when caching is off). */
 BYBYCU_API int bybycu_tune_cache_path(char* buf, int buf_len);
 
+/* ---- paged key/value cache and the operators around it ------------------------------------ */
+
+/* One layer's paged cache and the batch that a call works on.  K and V are bf16; the element
+ * (page, head, slot, d) of either is at page * page_stride + head * head_stride + slot *
+ * token_stride + d (strides in elements, multiples of 8, both tensors 16-byte aligned), so
+ * head-major and token-major pages are both served.
+ *   Sequence b has kv_lens[b] tokens in the cache, the last q_start[b+1] - q_start[b] of them
+ *   new; its token at position p is in slot p % page_size of page page_table[b][p / page_size].
+ *   New token t (a row of q, k, v) of sequence b is at position
+ *   kv_lens[b] - (q_start[b+1] - t); a token at a negative position is padding (it is not
+ *   appended and its output rows are zero), and a row that belongs to no sequence is left alone.
+ *   page_table, q_start and kv_lens are device memory and read by the kernels: a page id outside
+ *   [0, n_pages) or a position past max_pages * page_size is not accessed and records device
+ *   error 9. */
+typedef struct bybycu_paged_kv {
+    void* k;
+    void* v;
+    int64_t page_stride, head_stride, token_stride;
+    const int32_t* page_table;      /* [n_seqs, max_pages], rows table_stride apart */
+    int64_t table_stride;
+    const int32_t* q_start;         /* [n_seqs + 1], not decreasing */
+    const int32_t* kv_lens;         /* [n_seqs] */
+    int32_t n_pages, page_size, kv_heads, head_dim;   /* head_dim a multiple of 8, at most 256 */
+    int32_t max_pages, n_seqs, n_tokens;              /* n_tokens: rows of q (and k, v) */
+    int32_t reserved;               /* 0 */
+} bybycu_paged_kv;
+
+/* Rotary positions and the append of new keys and values, one launch: q and k of every new token
+ * are turned by its position, q_out receives the turned queries, the cache's slots of the new
+ * tokens the turned keys and the values (bf16, one rounding).  Dimension pair i of a head turns by
+ * position * turns[i] full turns (turns = frequency / 2 pi, fp64 on the device, so that the angle
+ * keeps fp32 accuracy at any position); the pairs are (i, i + pairs) of the first 2 * pairs
+ * dimensions, or with interleaved != 0 (2i, 2i + 1); dimensions from 2 * pairs on pass.  Turned
+ * values are multiplied by `magnitude` (1 but for frequency schemes that rescale).  Two new tokens
+ * must not share a slot.  Strides in elements; the last dimension is dense. */
+typedef struct bybycu_rope {
+    const void *q, *k, *v;          /* [n_tokens, q_heads | kv_heads | kv_heads, head_dim], in_dtype */
+    void* q_out;                    /* bf16 [n_tokens, q_heads, head_dim] */
+    int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+    int64_t out_token_stride, out_head_stride;
+    const double* turns;            /* [pairs], may be NULL when pairs = 0 */
+    const int32_t* positions;       /* [n_tokens] to turn by, or NULL: the positions in the cache */
+    int32_t in_dtype, q_heads, pairs, interleaved;
+    float magnitude;
+    int32_t reserved;               /* 0 */
+} bybycu_rope;
+BYBYCU_API int bybycu_rope_append(const bybycu_paged_kv* kv, const bybycu_rope* args, void* stream);
+
+/* Attention of the new tokens over the cache (which holds their own keys and values already):
+ *     s_ij = scale * q_i . k_j;   softcap > 0: s = softcap * tanh(s / softcap);
+ *     slopes: s -= slopes[head] * |p_i - j|;   out_i = sum_j softmax_j(s_ij) v_j
+ * over the positions j < kv_lens[b] with j <= p_i, or j < prefix_lens[b] where given, and, with
+ * window > 0, p_i - j < window.  A row that sees no key gives zeros.  q head h reads kv head
+ * h / (q_heads / kv_heads).  Cache slots past kv_lens[b] and pages that no new token sees are
+ * not used, whatever they hold.
+ *   max_q, max_kv bound the new tokens and the cache length of every sequence (the launch is sized
+ *   by them); a sequence beyond either records device error 10 and its rows beyond are not
+ *   computed.
+ *   route AUTO: GEMV (warp-level MMAs, the cache split over the grid) for few query rows a kv
+ *   head, TC (tcgen05) for more where the head dimension and page size allow, SIMT (one warp a
+ *   row, fp32) for head dimensions that no other kernel is built for.
+ * Scores, softmax statistics and sums are fp32; the probabilities enter the product with V as
+ * bf16 for a bf16 output and as two bf16 terms (16 bits) for an fp32 output. */
+typedef struct bybycu_attention {
+    const void* q;                  /* bf16 [n_tokens, q_heads, head_dim] */
+    void* out;                      /* out_dtype, same shape */
+    int64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride;
+    const float* slopes;            /* [q_heads] or NULL */
+    const int32_t* prefix_lens;     /* [n_seqs] or NULL */
+    int32_t out_dtype, q_heads, max_q, max_kv, window, route;
+    float scale, softcap;
+} bybycu_attention;
+BYBYCU_API int bybycu_paged_attention(const bybycu_paged_kv* kv, const bybycu_attention* args, void* stream);
+
+/* Copies pages within a cache, all layers of K and V in one launch (several for more than a
+ * thousand pairs): for each pair (src, dst) of the HOST array pairs[n_pairs][2] page dst becomes
+ * page src.  Page p of layer l is the page_bytes dense bytes at l * layer_stride + p * page_stride
+ * (bytes, multiples of 16, as the pointers are); v may be NULL.  The pairs act at once: no page
+ * may be the destination of one and a source or destination of another (BYBYCU_ERR_ARGS), so
+ * that the order of the copies cannot matter. */
+BYBYCU_API int bybycu_copy_pages(void* k, void* v, int n_layers, int64_t layer_stride, int64_t page_stride,
+                                 int64_t page_bytes, int n_pages, const int32_t* pairs, int n_pairs, void* stream);
+
+/* Beam search's selection: of the groups' beams * vocab continuations each the `keep` best by
+ * scores[g][b] + logits[row][t] - logsumexp(logits[row]), row = g * beams + b, best first, equal
+ * scores by the lower b, then the lower t.  A NaN sum (a row with no finite logit, with NaN or
+ * with +inf) counts as -inf.  logits F32 or BF16 [groups * beams, vocab], rows row_stride elements
+ * apart; scores fp32 [groups, beams]; the outputs [groups, keep].  1 <= keep <= 64, at most
+ * beams * vocab; beams <= 64. */
+BYBYCU_API int bybycu_beam_select(const void* logits, int logits_dtype, int64_t row_stride, const float* scores,
+                                  int groups, int beams, int vocab, int keep, float* out_scores,
+                                  int32_t* out_beams, int32_t* out_tokens, void* stream);
+
 /* Device-pointer twin of nimf_cpu_vm_run_slots (backends/cpu/cpu_kernels.h:118-121,
  * cpu_vm.c:178-182): runs a micro-VM program whose first op is OP_TILE_GEMM (formats
  * 0/1/2, followed by the canonical tile ops), OP_FP4_COOP_GEMM, OP_Q4_GEMV or
