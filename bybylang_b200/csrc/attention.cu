@@ -122,7 +122,7 @@ extern "C" int bybycu_paged_attention(const bybycu_paged_kv* kv, const bybycu_at
         return set_error(BYBYCU_ERR_SHAPE, "paged_attention: max_q=%d max_kv=%d window=%d", a->max_q, a->max_kv, a->window);
     if (!std::isfinite(a->scale) || !(a->softcap >= 0.0f) || !std::isfinite(a->softcap))
         return set_error(BYBYCU_ERR_ARGS, "paged_attention: scale %g, softcap %g", a->scale, a->softcap);
-    if (a->route != BYBYCU_ROUTE_AUTO && a->route != BYBYCU_ROUTE_SIMT)
+    if (a->route != BYBYCU_ROUTE_AUTO && a->route != BYBYCU_ROUTE_SIMT && a->route != BYBYCU_ROUTE_GEMV)
         return set_error(BYBYCU_ERR_ARGS, "unknown route %d", a->route);
     if (c.n_tokens == 0 || c.n_seqs == 0) return BYBYCU_OK;
     if (!a->q || !a->out) return set_error(BYBYCU_ERR_ARGS, "paged_attention: a slot is missing");
@@ -136,5 +136,7 @@ extern "C" int bybycu_paged_attention(const bybycu_paged_kv* kv, const bybycu_at
                          a->q_heads / c.kv_heads, a->max_q, a->max_kv, a->window, a->scale * attn::kLog2e, a->softcap,
                          a->softcap > 0.0f ? a->scale / a->softcap : 0.0f};
     const bool mod = a->softcap > 0.0f || a->slopes, f32 = a->out_dtype == BYBYCU_DT_F32;
-    return attn::launch_simt(c, p, mod, f32, static_cast<cudaStream_t>(stream));
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (a->route == BYBYCU_ROUTE_SIMT) return attn::launch_simt(c, p, mod, f32, s);
+    return attn::launch_gemv(c, p, f32, s);
 }

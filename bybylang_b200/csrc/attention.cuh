@@ -77,5 +77,18 @@ __device__ __forceinline__ int64_t slot_of(const kvc::Cache& c, int b, int j) {
     return id * c.page_stride + (j - pg * c.page_size) * c.token_stride;
 }
 
+// Four dimensions of a finished row: sums over their total, zeros for a row that saw nothing.
+template <bool F32>
+__device__ __forceinline__ void store_row4(const Params& p, int64_t token, int64_t head, int d, float4 acc, float sum) {
+    const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
+    const int64_t at = token * p.o_token + head * p.o_head + d;
+    if constexpr (F32) {
+        *reinterpret_cast<float4*>(static_cast<float*>(p.out) + at) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+    } else {
+        __nv_bfloat162 h[2] = {__floats2bfloat162_rn(acc.x * inv, acc.y * inv), __floats2bfloat162_rn(acc.z * inv, acc.w * inv)};
+        *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.out) + at) = *reinterpret_cast<const uint2*>(h);
+    }
+}
+
 }  // namespace attn
 }  // namespace bybycu

@@ -1,0 +1,511 @@
+// attn_gemv.cu - the GEMV route of paged attention: few query rows a kv head over a long cache.
+//
+// At one token and a group of G query heads the work is 4 G flop for every 4 bytes of K and V, so
+// the cache's stream from HBM is all there is (6.5 TB/s; at G = 8 that is 52 TFLOP/s, above what
+// fp32 FMAs with their conversions keep up with), and warp-level bf16 MMAs (m16n8k16) with the
+// group's rows as M take it along.
+//
+//   * A CTA is WK key groups of WM warps; a warp holds 16 query rows, a group streams its own
+//     chunks of KC = 16 WM keys through its own cp.async ring, so that no barrier joins the groups
+//     until the end.  WM = 1 for up to 16 rows, 2 and 4 above (rows then share the chunk).
+//   * Keys come through the page table, a 16-byte piece of a slot per copy; slots outside the
+//     rows' common range and pages that do not exist are filled with zeros instead of read.
+//   * Every warp keeps the running maximum and sum of its rows (online softmax); scores and
+//     probabilities stay in registers: the accumulator layout of S is the A layout of P.
+//   * fp32 output: P enters as three bf16 terms (24 bits), so the product with V is exact to fp32
+//     rounding; bf16 output: one rounding.
+//   * The cache axis is cut over the grid as well (splits of whole chunks); each split leaves
+//     unnormalised sums with their maximum, and a second, dependent launch joins them in a fixed
+//     order.
+#include <algorithm>
+
+#include "attention.cuh"
+
+namespace bybycu {
+
+static int scratch_pool(int device, cudaMemPool_t* pool);
+
+namespace attn {
+
+// What a split leaves for the joining kernel: row = (token * q_heads + head).
+struct Partials {
+    float* o;        // [splits][tokens * q_heads][head_dim]
+    float2* ml;      // [splits][tokens * q_heads]: maximum (log2 units) and sum
+    int64_t rows;
+};
+
+// The keys that a tile of `rows` rows (row r: token r / group, head r % group) can see, aligned
+// down to the chunk grid, and how many splits of split_keys they take.
+struct TileRange {
+    int lo, hi, lo_aligned, splits;
+};
+__device__ __forceinline__ TileRange tile_range(const Params& p, const Seq& s, int first_row, int rows, int align,
+                                                int split_keys) {
+    TileRange r{0, 0, 0, 1};
+    const int t0 = first_row / p.group, t1 = (first_row + rows - 1) / p.group;
+    int lo0, hi0, lo1, hi1;
+    row_range(p, s, s.first_pos + t0, &lo0, &hi0);
+    row_range(p, s, s.first_pos + t1, &lo1, &hi1);
+    // rows at negative positions see nothing and come first
+    if (hi1 <= 0) return r;
+    r.lo = hi0 > 0 ? lo0 : 0;
+    r.hi = hi1;
+    r.lo_aligned = r.lo / align * align;
+    r.splits = max(1, (r.hi - r.lo_aligned + split_keys - 1) / split_keys);
+    return r;
+}
+
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                 "{%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// 16 bytes from src, or zeros.
+__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, bool real) {
+    const int n = real ? 16 : 0;
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float bf16_lo(uint32_t u) { return __uint_as_float(u << 16); }
+__device__ __forceinline__ float bf16_hi(uint32_t u) { return __uint_as_float(u & 0xffff0000u); }
+
+template <int HD, int WM>
+struct GemvCfg {
+    static constexpr int kWarps = 4;
+    static constexpr int kWK = kWarps / WM;
+    static constexpr int kKC = 16 * WM;                          // keys of a chunk
+    static constexpr int kPitch = HD * 2 + 16;                   // a row's bytes: 16 more keep ldmatrix free of conflicts
+    static constexpr int kTensorBytes = kKC * kPitch;            // one chunk of K or of V
+    static constexpr int kChunkBytes = 2 * kTensorBytes;
+    // about 100 KB, so that two CTAs share an SM, but three chunks a group (two where three do not fit)
+    static constexpr int kQBytes = HD > 128 ? 16 * WM * kPitch : 0;
+    static constexpr int kFit = 104 * 1024 / (kWK * kChunkBytes);
+    static constexpr int kLeast = 3 * kWK * kChunkBytes + kQBytes <= 227 * 1024 ? 3 : 2;
+    static constexpr int kStages = kFit < kLeast ? kLeast : kFit > 8 ? 8 : kFit;
+    static constexpr int kRingBytes = kWK * kStages * kChunkBytes;
+    // the end: every warp's sums [16][HD] fp32 and statistics, in the ring's place
+    static constexpr int kJoinBytes = kWarps * 16 * HD * 4;
+    static constexpr int kSmem = (kRingBytes > kJoinBytes ? kRingBytes : kJoinBytes) + kQBytes;
+    static_assert(kSmem <= 227 * 1024, "shared memory");
+};
+
+template <int HD, int WM, bool F32>
+__global__ void __launch_bounds__(128) attention_gemv_kernel(const kvc::Cache c, const Params p, const Partials part,
+                                                             int split_keys, int row_tiles) {
+    using C = GemvCfg<HD, WM>;
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ float s_m[4][16], s_l[4][16];
+    pdl_launch_dependents();
+    pdl_wait();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+    const int wm = warp % WM, wk = warp / WM;
+    const int kvh = blockIdx.y / row_tiles, first_row = blockIdx.y % row_tiles * (16 * WM), b = blockIdx.z, split = blockIdx.x;
+    const Seq s = load_seq(c, p, b);
+    const int rows = min(16 * WM, s.rows * p.group - first_row);
+    if (rows <= 0) return;
+    const TileRange range = tile_range(p, s, first_row, rows, 16, split_keys);
+    if (split >= range.splits) return;
+    const int seg_lo = range.lo_aligned + split * split_keys;
+    const int seg_hi = range.splits == 1 ? range.hi : min(range.hi, seg_lo + split_keys);
+    const int D = c.head_dim;
+
+    // this thread's two rows of its warp's sixteen
+    int row_lo[2], row_hi[2], row_pos[2];
+    float slope[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int r = wm * 16 + g + 8 * i;
+        row_pos[i] = s.first_pos + (first_row + r) / p.group;
+        row_lo[i] = row_hi[i] = 0;
+        slope[i] = 0.0f;
+        if (r < rows) {
+            row_range(p, s, row_pos[i], &row_lo[i], &row_hi[i]);
+            if (p.slopes) slope[i] = p.slopes[kvh * p.group + (first_row + r) % p.group] * kLog2e;
+        }
+    }
+    const bool mod = p.cap > 0.0f || p.slopes;
+    // keys that every row of the warp sees need no mask
+    int all_lo = max(row_lo[0], row_lo[1]), all_hi = min(row_hi[0], row_hi[1]);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        all_lo = max(all_lo, __shfl_xor_sync(~0u, all_lo, o));
+        all_hi = min(all_hi, __shfl_xor_sync(~0u, all_hi, o));
+    }
+
+    // Q as A fragments: registers up to 128 dimensions, shared memory above
+    constexpr int kSteps = HD / 16;
+    uint32_t qf[HD > 128 ? 1 : kSteps][4];
+    const uint32_t ring = smem_u32(smem), qs = ring + (C::kSmem - C::kQBytes);
+    if constexpr (HD > 128) {
+        for (int i = threadIdx.x; i < 16 * WM * (HD / 8); i += 128) {
+            const int r = i / (HD / 8), d = i % (HD / 8) * 8;
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (r < rows && d < D)
+                v = *reinterpret_cast<const uint4*>(p.q + (s.q0 + (first_row + r) / p.group) * p.q_token +
+                                                    (kvh * p.group + (first_row + r) % p.group) * p.q_head + d);
+            *reinterpret_cast<uint4*>(smem + (C::kSmem - C::kQBytes) + r * C::kPitch + d * 2) = v;
+        }
+        __syncthreads();
+    } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int r = wm * 16 + g + 8 * i;
+            const __nv_bfloat16* q = p.q + (s.q0 + (first_row + r) / p.group) * p.q_token +
+                                     (kvh * p.group + (first_row + r) % p.group) * p.q_head;
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int d = k * 16 + e * 8 + t4 * 2;
+                    qf[k][e * 2 + i] = r < rows && d < D ? *reinterpret_cast<const uint32_t*>(q + d) : 0u;
+                }
+        }
+    }
+
+    // the group's chunks: wk, wk + WK, ... of the segment
+    const int n_all = seg_hi > seg_lo ? (seg_hi - seg_lo + C::kKC - 1) / C::kKC : 0;
+    const int n_mine = n_all > wk ? (n_all - wk + C::kWK - 1) / C::kWK : 0;
+    const uint32_t my_ring = ring + wk * C::kStages * C::kChunkBytes;
+    const int gt = wm * 32 + lane;   // thread of the group
+    const int32_t* table = c.page_table + b * c.table_stride;
+    const int64_t head_off = static_cast<int64_t>(kvh) * c.head_stride;
+    // One slot row is HD / 8 pieces of 16 bytes; a thread copies the same piece of every
+    // (32 WM / pieces)-th slot.
+    constexpr int kPieces = HD / 8, kRowStep = 32 * WM / kPieces;
+    static_assert(kRowStep >= 1 && C::kKC % kRowStep == 0, "copy layout");
+    const int piece = gt % kPieces, row0 = gt / kPieces;
+    const bool piece_real = piece * 8 < D;
+    auto fetch = [&](int i) {
+        if (i < n_mine) {
+            const int j0 = seg_lo + (wk + i * C::kWK) * C::kKC;
+            const uint32_t dst = my_ring + i % C::kStages * C::kChunkBytes + row0 * C::kPitch + piece * 16;
+            int pg_have = -1, id = -1;
+#pragma unroll
+            for (int r = 0; r < C::kKC / kRowStep; ++r) {
+                const int j = j0 + row0 + r * kRowStep;
+                const bool in = j >= range.lo && j < seg_hi;
+                const int pg = in ? j / c.page_size : -1;
+                if (in && pg != pg_have) {
+                    id = table[pg];
+                    pg_have = pg;
+                    if (id < 0 || id >= c.n_pages) {
+                        record_device_error(kDevErrPage);
+                        id = -1;
+                    }
+                }
+                const bool real = in && id >= 0 && piece_real;
+                const int64_t at = real ? id * c.page_stride + (j - pg * c.page_size) * c.token_stride + head_off + piece * 8 : 0;
+                cp_async16_or_zero(dst + r * kRowStep * C::kPitch, c.k + at, real);
+                cp_async16_or_zero(dst + C::kTensorBytes + r * kRowStep * C::kPitch, c.v + at, real);
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    auto group_sync = [&]() {
+        if constexpr (WM == 1) __syncwarp();
+        else named_barrier(1 + wk, 32 * WM);
+    };
+
+    float o[HD / 8][4] = {};
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < C::kStages - 1; ++i) fetch(i);
+    for (int i = 0; i < n_mine; ++i) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(C::kStages - 2) : "memory");
+        group_sync();   // the chunk is whole, and the slot that the next fetch fills is free
+        fetch(i + C::kStages - 1);
+        const int j0 = seg_lo + (wk + i * C::kWK) * C::kKC;
+        const uint32_t kc = my_ring + i % C::kStages * C::kChunkBytes, vc = kc + C::kTensorBytes;
+        float sc[C::kKC / 8][4] = {};
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) {
+            uint32_t a[4];
+            if constexpr (HD > 128) ldsm4(qs + (wm * 16 + (lane & 15)) * C::kPitch + k * 32 + (lane >> 4) * 16, a);
+            else { a[0] = qf[k][0]; a[1] = qf[k][1]; a[2] = qf[k][2]; a[3] = qf[k][3]; }
+#pragma unroll
+            for (int n = 0; n < C::kKC / 16; ++n) {
+                uint32_t kf[4];
+                ldsm4(kc + (n * 16 + (lane >> 4) * 8 + (lane & 7)) * C::kPitch + k * 32 + ((lane >> 3) & 1) * 16, kf);
+                mma_bf16(sc[2 * n], a, kf[0], kf[1]);
+                mma_bf16(sc[2 * n + 1], a, kf[2], kf[3]);
+            }
+        }
+        const bool masked = j0 < all_lo || j0 + C::kKC > all_hi;
+#pragma unroll
+        for (int n = 0; n < C::kKC / 8; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int j = j0 + n * 8 + t4 * 2 + (e & 1), r = e >> 1;
+                if (mod) sc[n][e] = score_log2<true>(p, sc[n][e], slope[r], row_pos[r] - j);
+                else sc[n][e] *= p.scale_log2;
+                if (masked && (j < row_lo[r] || j >= row_hi[r])) sc[n][e] = -INFINITY;
+            }
+        float mn[2] = {m[0], m[1]};
+#pragma unroll
+        for (int n = 0; n < C::kKC / 8; ++n) {
+            mn[0] = fmaxf(mn[0], fmaxf(sc[n][0], sc[n][1]));
+            mn[1] = fmaxf(mn[1], fmaxf(sc[n][2], sc[n][3]));
+        }
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            mn[r] = fmaxf(mn[r], __shfl_xor_sync(~0u, mn[r], 1));
+            mn[r] = fmaxf(mn[r], __shfl_xor_sync(~0u, mn[r], 2));
+        }
+        float base[2], keep[2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            base[r] = mn[r] == -INFINITY ? 0.0f : mn[r];
+            keep[r] = exp2f(m[r] - base[r]);
+        }
+        if (__any_sync(~0u, mn[0] != m[0] || mn[1] != m[1])) {
+#pragma unroll
+            for (int n = 0; n < HD / 8; ++n) {
+                o[n][0] *= keep[0];
+                o[n][1] *= keep[0];
+                o[n][2] *= keep[1];
+                o[n][3] *= keep[1];
+            }
+            l[0] *= keep[0];
+            l[1] *= keep[1];
+            m[0] = mn[0];
+            m[1] = mn[1];
+        }
+#pragma unroll
+        for (int n = 0; n < C::kKC / 8; ++n) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[n][e] = exp2f(sc[n][e] - base[e >> 1]);
+            l[0] += sc[n][0] + sc[n][1];
+            l[1] += sc[n][2] + sc[n][3];
+        }
+#pragma unroll
+        for (int n = 0; n < C::kKC / 16; ++n) {
+            constexpr int kTerms = F32 ? 3 : 1;
+            uint32_t pf[kTerms][4];
+#pragma unroll
+            for (int f = 0; f < 4; ++f) {   // a0 a1: keys 0-7 (rows g, g + 8); a2 a3: keys 8-15
+                float x = sc[2 * n + (f >> 1)][(f & 1) * 2], y = sc[2 * n + (f >> 1)][(f & 1) * 2 + 1];
+#pragma unroll
+                for (int w = 0; w < kTerms; ++w) {
+                    pf[w][f] = pack_bf16(x, y);
+                    x -= bf16_lo(pf[w][f]);
+                    y -= bf16_hi(pf[w][f]);
+                }
+            }
+#pragma unroll
+            for (int d = 0; d < HD / 16; ++d) {
+                uint32_t vf[4];
+                ldsm4_t(vc + (n * 16 + ((lane >> 3) & 1) * 8 + (lane & 7)) * C::kPitch + d * 32 + (lane >> 4) * 16, vf);
+#pragma unroll
+                for (int w = 0; w < kTerms; ++w) {
+                    mma_bf16(o[2 * d], pf[w], vf[0], vf[1]);
+                    mma_bf16(o[2 * d + 1], pf[w], vf[2], vf[3]);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        l[r] += __shfl_xor_sync(~0u, l[r], 1);
+        l[r] += __shfl_xor_sync(~0u, l[r], 2);
+    }
+    // join the key groups: every warp's sums into shared memory, in the ring's place
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();
+    float* so = reinterpret_cast<float*>(smem);   // [warp][16][HD]
+    if (t4 == 0) {
+        s_m[warp][g] = m[0]; s_m[warp][g + 8] = m[1];
+        s_l[warp][g] = l[0]; s_l[warp][g + 8] = l[1];
+    }
+#pragma unroll
+    for (int n = 0; n < HD / 8; ++n) {
+        *reinterpret_cast<float2*>(so + (warp * 16 + g) * HD + n * 8 + t4 * 2) = make_float2(o[n][0], o[n][1]);
+        *reinterpret_cast<float2*>(so + (warp * 16 + g + 8) * HD + n * 8 + t4 * 2) = make_float2(o[n][2], o[n][3]);
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < rows * (HD / 4); i += 128) {
+        const int r = i / (HD / 4), d = i % (HD / 4) * 4, w0 = r / 16, rr = r % 16;
+        if (d >= D) continue;
+        float mx = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < C::kWK; ++k) mx = fmaxf(mx, s_m[k * WM + w0][rr]);
+        const float base = mx == -INFINITY ? 0.0f : mx;
+        float sum = 0.0f;
+        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int k = 0; k < C::kWK; ++k) {
+            const int w = k * WM + w0;
+            const float f = exp2f(s_m[w][rr] - base);
+            const float4 v = *reinterpret_cast<const float4*>(so + (w * 16 + rr) * HD + d);
+            sum = fmaf(f, s_l[w][rr], sum);
+            acc.x = fmaf(f, v.x, acc.x);
+            acc.y = fmaf(f, v.y, acc.y);
+            acc.z = fmaf(f, v.z, acc.z);
+            acc.w = fmaf(f, v.w, acc.w);
+        }
+        const int64_t token = s.q0 + (first_row + r) / p.group, head = kvh * p.group + (first_row + r) % p.group;
+        if (range.splits > 1) {
+            const int64_t at = split * part.rows + token * p.q_heads + head;
+            *reinterpret_cast<float4*>(part.o + at * D + d) = acc;
+            if (d == 0) part.ml[at] = make_float2(mx, sum);
+            continue;
+        }
+        store_row4<F32>(p, token, head, d, acc, sum);
+    }
+}
+
+// Joins the splits: one warp a row (token, head), splits in order.
+template <bool F32>
+__global__ void __launch_bounds__(128) attention_join_kernel(const kvc::Cache c, const Params p, const Partials part,
+                                                             int split_keys, int tile_rows) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int lane = threadIdx.x & 31;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+    if (row >= part.rows) return;
+    const int t = static_cast<int>(row / p.q_heads), h = static_cast<int>(row % p.q_heads), D = c.head_dim;
+    int b = 0;
+    for (int i = 0; i < c.n_seqs; i += 32) b += __popc(__ballot_sync(~0u, i + lane < c.n_seqs && c.q_start[i + lane + 1] <= t));
+    if (b >= c.n_seqs || t < c.q_start[0]) return;
+    const Seq s = load_seq(c, p, b);
+    if (t - s.q0 >= s.rows) return;
+    const int first_row = ((t - s.q0) * p.group + h % p.group) / tile_rows * tile_rows;
+    const TileRange range = tile_range(p, s, first_row, min(tile_rows, s.rows * p.group - first_row), 16, split_keys);
+    if (range.splits == 1) return;   // written by the first kernel
+    float mx = -INFINITY;
+    for (int k = lane; k < range.splits; k += 32) mx = fmaxf(mx, part.ml[k * part.rows + row].x);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, o));
+    const float base = mx == -INFINITY ? 0.0f : mx;
+    for (int d = lane * 4; d < D; d += 128) {
+        float sum = 0.0f;
+        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+        for (int k = 0; k < range.splits; ++k) {
+            const float2 ml = part.ml[k * part.rows + row];
+            const float4 v = *reinterpret_cast<const float4*>(part.o + (k * part.rows + row) * D + d);
+            const float f = exp2f(ml.x - base);
+            sum = fmaf(f, ml.y, sum);
+            acc.x = fmaf(f, v.x, acc.x);
+            acc.y = fmaf(f, v.y, acc.y);
+            acc.z = fmaf(f, v.z, acc.z);
+            acc.w = fmaf(f, v.w, acc.w);
+        }
+        store_row4<F32>(p, t, h, d, acc, sum);
+    }
+}
+
+// The launch of a route's kernel and, where the grid splits the cache, of the joining one.
+static cudaLaunchConfig_t pdl_config(dim3 grid, int threads, size_t smem, cudaStream_t stream, cudaLaunchAttribute* attr) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    attr->id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr->val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cfg;
+}
+
+static int launch_join(const kvc::Cache& c, const Params& p, const Partials& part, int split_keys, int tile_rows, bool f32,
+                       cudaStream_t stream) {
+    cudaLaunchAttribute attr[1];
+    const cudaLaunchConfig_t cfg = pdl_config(dim3(static_cast<unsigned>(ceil_div(part.rows, 4))), 128, 0, stream, attr);
+    BYBYCU_CUDA_TRY(cudaLaunchKernelEx(&cfg, f32 ? attention_join_kernel<true> : attention_join_kernel<false>, c, p, part,
+                                       split_keys, tile_rows));
+    return BYBYCU_OK;
+}
+
+// Scratch of a split launch, stream-ordered.
+struct SplitScratchMem {
+    void* ptr = nullptr;
+    cudaStream_t stream = nullptr;
+    int take(int device, int64_t rows, int splits, int dim, cudaStream_t s, Partials* part) {
+        cudaMemPool_t pool = nullptr;
+        if (int rc = scratch_pool(device, &pool)) return rc;
+        const size_t o_bytes = static_cast<size_t>(rows) * splits * dim * 4;
+        BYBYCU_CUDA_TRY(cudaMallocFromPoolAsync(&ptr, o_bytes + static_cast<size_t>(rows) * splits * 8, pool, s));
+        stream = s;
+        part->o = static_cast<float*>(ptr);
+        part->ml = reinterpret_cast<float2*>(static_cast<char*>(ptr) + o_bytes);
+        part->rows = rows;
+        return BYBYCU_OK;
+    }
+    ~SplitScratchMem() {
+        if (ptr) cudaFreeAsync(ptr, stream);
+    }
+};
+
+// The longest stretch of keys that one row tile can visit.
+static int64_t longest_span(const Params& p, int tile_rows) {
+    int64_t span = p.max_kv;
+    if (p.window > 0 && !p.prefix) span = std::min<int64_t>(span, static_cast<int64_t>(p.window) + ceil_div(tile_rows, p.group) + 16);
+    return std::max<int64_t>(span, 1);
+}
+
+template <int HD, int WM, bool F32>
+static int launch_gemv_tile(const kvc::Cache& c, const Params& p, const DeviceInfo& info, cudaStream_t stream) {
+    using C = GemvCfg<HD, WM>;
+    auto kern = attention_gemv_kernel<HD, WM, F32>;
+    static std::once_flag once[64];
+    static cudaError_t prep[64];
+    if (info.device < 0 || info.device >= 64) return set_error(BYBYCU_ERR_ARGS, "device %d out of range", info.device);
+    std::call_once(once[info.device], [&] {
+        prep[info.device] = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+    });
+    if (prep[info.device] != cudaSuccess) return cuda_fail(prep[info.device], "attention_gemv_kernel shared memory");
+    const int row_tiles = static_cast<int>(ceil_div(static_cast<int64_t>(p.max_q) * p.group, 16 * WM));
+    if (static_cast<int64_t>(row_tiles) * c.kv_heads > 65535 || c.n_seqs > 65535)
+        return set_error(BYBYCU_ERR_SHAPE, "paged_attention: %d sequences, %d kv heads, %d new tokens", c.n_seqs, c.kv_heads, p.max_q);
+    const int64_t units = static_cast<int64_t>(row_tiles) * c.kv_heads * c.n_seqs;
+    const int slots = info.sm_count * (C::kSmem <= 113 * 1024 ? 2 : 1);
+    const int64_t span = longest_span(p, 16 * WM);
+    // One sequence: as many splits as fill the card once.  More: their lengths may differ up to
+    // the longest, so pieces of a sixth of a CTA's share of half of the most there can be, whatever
+    // the lengths, keep the tail short.  256 keys at least: below, a split's own sums weigh.
+    const int64_t share = c.n_seqs == 1 ? ceil_div(span * units, slots) : ceil_div(span * units, 12 * slots);
+    const int split_keys = static_cast<int>(std::min<int64_t>(std::max<int64_t>(ceil_div(share, 64) * 64, 256), INT32_MAX / 2 / 64 * 64));
+    const int splits = static_cast<int>(ceil_div(span + 16, split_keys));
+    Partials part{};
+    SplitScratchMem scratch;
+    if (splits > 1)
+        if (int rc = scratch.take(info.device, static_cast<int64_t>(c.n_tokens) * p.q_heads, splits, c.head_dim, stream, &part)) return rc;
+    cudaLaunchAttribute attr[1];
+    const cudaLaunchConfig_t cfg = pdl_config(dim3(static_cast<unsigned>(splits), static_cast<unsigned>(row_tiles * c.kv_heads),
+                                                   static_cast<unsigned>(c.n_seqs)), 128, C::kSmem, stream, attr);
+    BYBYCU_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, c, p, part, split_keys, row_tiles));
+    return splits > 1 ? launch_join(c, p, part, split_keys, 16 * WM, F32, stream) : BYBYCU_OK;
+}
+
+template <int HD, bool F32>
+static int launch_gemv_rows(const kvc::Cache& c, const Params& p, const DeviceInfo& info, cudaStream_t stream) {
+    const int64_t rows = static_cast<int64_t>(p.max_q) * p.group;
+    if (rows <= 16) return launch_gemv_tile<HD, 1, F32>(c, p, info, stream);
+    if (rows <= 32) return launch_gemv_tile<HD, 2, F32>(c, p, info, stream);
+    return launch_gemv_tile<HD, 4, F32>(c, p, info, stream);
+}
+
+static int launch_gemv(const kvc::Cache& c, const Params& p, bool f32, cudaStream_t stream) {
+    if (p.max_q == 0) return BYBYCU_OK;
+    DeviceInfo info;
+    if (int rc = current_device_info(&info)) return rc;
+    if (c.head_dim <= 64) return f32 ? launch_gemv_rows<64, true>(c, p, info, stream) : launch_gemv_rows<64, false>(c, p, info, stream);
+    if (c.head_dim <= 128) return f32 ? launch_gemv_rows<128, true>(c, p, info, stream) : launch_gemv_rows<128, false>(c, p, info, stream);
+    return f32 ? launch_gemv_rows<256, true>(c, p, info, stream) : launch_gemv_rows<256, false>(c, p, info, stream);
+}
+
+}  // namespace attn
+}  // namespace bybycu

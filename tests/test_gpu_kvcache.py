@@ -48,7 +48,7 @@ DECODE = [(1, n) for n in (1, 2, 15, 16, 17, 63, 64, 65, 127, 128, 129, 500, 0)]
 
 
 @pytest.mark.parametrize("out_dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("route", [AUTO, SIMT])
+@pytest.mark.parametrize("route", [AUTO, GEMV, SIMT])
 @pytest.mark.parametrize("dim,page,heads,kv_heads", [(64, 16, 8, 2), (128, 64, 4, 4), (128, 16, 8, 1), (8, 1, 3, 1),
                                                      (80, 7, 6, 2), (96, 48, 5, 5), (256, 128, 2, 1), (40, 256, 4, 2)])
 @pytest.mark.parametrize("lens", [RAGGED, DECODE], ids=["ragged", "decode"])
@@ -66,7 +66,7 @@ MODS = [dict(softcap=5.0), dict(softcap=30.0, window=40), dict(window=1), dict(w
         dict(slopes=True), dict(slopes=True, softcap=20.0, prefix=[37] * 8, window=100), dict(scale=0.0), dict(scale=-0.3)]
 
 
-@pytest.mark.parametrize("route", [AUTO, SIMT])
+@pytest.mark.parametrize("route", [AUTO, GEMV, SIMT])
 @pytest.mark.parametrize("dim,page,heads,kv_heads", [(64, 16, 8, 2), (128, 64, 4, 4), (80, 7, 6, 2), (128, 32, 24, 1)])
 @pytest.mark.parametrize("mods", MODS, ids=lambda m: "-".join(m))
 def test_attention_masks_and_scores(mods, dim, page, heads, kv_heads, route):
@@ -81,7 +81,7 @@ def test_attention_masks_and_scores(mods, dim, page, heads, kv_heads, route):
     check(Batch(DECODE, page=page, heads=heads, kv_heads=kv_heads, dim=dim, seed=4), route, **one)
 
 
-@pytest.mark.parametrize("route", [AUTO, SIMT])
+@pytest.mark.parametrize("route", [AUTO, GEMV, SIMT])
 @pytest.mark.parametrize("lens", [[(1, 400), (1, 90)], [(40, 400), (200, 390)]], ids=["decode", "chunk"])
 def test_attention_pages_before_the_window_are_gone(lens, route):
     """A freed page (-1 in the table, its memory someone else's NaN) before the window is not touched."""
@@ -95,7 +95,7 @@ def test_attention_pages_before_the_window_are_gone(lens, route):
     check(bt, route, window=50)
 
 
-@pytest.mark.parametrize("route", [AUTO, SIMT])
+@pytest.mark.parametrize("route", [AUTO, GEMV, SIMT])
 def test_attention_large_scores(route):
     """Scores in the hundreds: the running maximum carries the sums, whatever order the keys come in."""
     bt = Batch([(1, 700), (70, 700)], page=64, heads=4, kv_heads=1, dim=64, seed=5, spread=40.0)
