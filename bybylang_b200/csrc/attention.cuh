@@ -47,6 +47,12 @@ __device__ __forceinline__ void row_range(const Params& p, const Seq& s, int pos
     *lo = p.window > 0 ? max(0, pos - p.window + 1) : 0;
 }
 
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 // The score of a pair in units of log2: raw = q . k.
 //   MOD: a tanh cap and / or distance slopes.  tanh(y) = 1 - 2 / (1 + e^2y) with the hardware's
 //   exponential and reciprocal: its absolute error is a few 2^-24, times the cap.
@@ -58,7 +64,7 @@ __device__ __forceinline__ float score_log2(const Params& p, float raw, float sl
         float s;
         if (p.cap > 0.0f) {
             const float y = raw * p.scale_over_cap;
-            s = p.cap * kLog2e * (1.0f - __fdividef(2.0f, 1.0f + exp2f(2.0f * kLog2e * y)));
+            s = p.cap * kLog2e * (1.0f - __fdividef(2.0f, 1.0f + ex2(2.0f * kLog2e * y)));
         } else {
             s = raw * p.scale_log2;
         }

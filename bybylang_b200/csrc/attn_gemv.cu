@@ -101,7 +101,9 @@ struct GemvCfg {
     static_assert(kSmem <= 227 * 1024, "shared memory");
 };
 
-template <int HD, int WM, bool F32>
+// P16: pages of whole 16-slot granules.  The address of a granule is then looked up once, 32
+// granules at a time and a batch ahead, so that no copy waits for the page table.
+template <int HD, int WM, bool F32, bool P16>
 __global__ void __launch_bounds__(128) attention_gemv_kernel(const kvc::Cache c, const Params p, const Partials part,
                                                              int split_keys, int row_tiles) {
     using C = GemvCfg<HD, WM>;
@@ -184,31 +186,72 @@ __global__ void __launch_bounds__(128) attention_gemv_kernel(const kvc::Cache c,
     // One slot row is HD / 8 pieces of 16 bytes; a thread copies the same piece of every
     // (32 WM / pieces)-th slot.
     constexpr int kPieces = HD / 8, kRowStep = 32 * WM / kPieces;
-    static_assert(kRowStep >= 1 && C::kKC % kRowStep == 0, "copy layout");
+    static_assert(kRowStep >= 1 && 16 % kRowStep == 0, "copy layout");
     const int piece = gt % kPieces, row0 = gt / kPieces;
     const bool piece_real = piece * 8 < D;
+    // The copies of chunk i into its ring slot, one commit group.  Chunks are fetched in order.
+    constexpr int kBatch = 32 / WM;   // chunks whose granules' pages one batch of lanes looks up
+    int batch_id = -1, next_id = -1;
+    auto granule_key = [&](int batch) {   // the first key of this lane's granule of a batch
+        return seg_lo + (wk + (batch * kBatch + lane / WM) * C::kWK) * C::kKC + lane % WM * 16;
+    };
+    auto look_up = [&](int batch) {
+        const int j = granule_key(batch);
+        return j < seg_hi && j + 16 > range.lo ? table[j / c.page_size] : 0;
+    };
+    if constexpr (P16) {
+        if (n_mine > 0) next_id = look_up(0);
+    }
+    int64_t granule = -1;   // this lane's granule: element offset of its first slot, -1 without one
     auto fetch = [&](int i) {
         if (i < n_mine) {
             const int j0 = seg_lo + (wk + i * C::kWK) * C::kKC;
             const uint32_t dst = my_ring + i % C::kStages * C::kChunkBytes + row0 * C::kPitch + piece * 16;
-            int pg_have = -1, id = -1;
-#pragma unroll
-            for (int r = 0; r < C::kKC / kRowStep; ++r) {
-                const int j = j0 + row0 + r * kRowStep;
-                const bool in = j >= range.lo && j < seg_hi;
-                const int pg = in ? j / c.page_size : -1;
-                if (in && pg != pg_have) {
-                    id = table[pg];
-                    pg_have = pg;
-                    if (id < 0 || id >= c.n_pages) {
-                        record_device_error(kDevErrPage);
-                        id = -1;
+            if constexpr (P16) {
+                if (i % kBatch == 0) {
+                    batch_id = next_id;
+                    const int j = granule_key(i / kBatch);
+                    const bool in = j < seg_hi && j + 16 > range.lo;
+                    if (batch_id < 0 || batch_id >= c.n_pages) {
+                        if (in) record_device_error(kDevErrPage);
+                        batch_id = -1;
                     }
+                    granule = in && batch_id >= 0 ? batch_id * c.page_stride + j % c.page_size * c.token_stride : -1;
+                    if (i + kBatch < n_mine) next_id = look_up(i / kBatch + 1);
                 }
-                const bool real = in && id >= 0 && piece_real;
-                const int64_t at = real ? id * c.page_stride + (j - pg * c.page_size) * c.token_stride + head_off + piece * 8 : 0;
-                cp_async16_or_zero(dst + r * kRowStep * C::kPitch, c.k + at, real);
-                cp_async16_or_zero(dst + C::kTensorBytes + r * kRowStep * C::kPitch, c.v + at, real);
+                int64_t at[WM];
+#pragma unroll
+                for (int w = 0; w < WM; ++w) at[w] = __shfl_sync(~0u, granule, i % kBatch * WM + w);
+                const bool whole = j0 >= range.lo && j0 + C::kKC <= seg_hi;
+#pragma unroll
+                for (int r = 0; r < C::kKC / kRowStep; ++r) {
+                    const int j = row0 + r * kRowStep;   // its granule is r * kRowStep / 16: kRowStep divides 16
+                    const int64_t base = at[r * kRowStep / 16];
+                    const bool real = base >= 0 && piece_real && (whole || (j0 + j >= range.lo && j0 + j < seg_hi));
+                    const int64_t off = real ? base + j % 16 * c.token_stride + head_off + piece * 8 : 0;
+                    cp_async16_or_zero(dst + r * kRowStep * C::kPitch, c.k + off, real);
+                    cp_async16_or_zero(dst + C::kTensorBytes + r * kRowStep * C::kPitch, c.v + off, real);
+                }
+            } else {
+                int pg_have = -1, id = -1;
+#pragma unroll
+                for (int r = 0; r < C::kKC / kRowStep; ++r) {
+                    const int j = j0 + row0 + r * kRowStep;
+                    const bool in = j >= range.lo && j < seg_hi;
+                    const int pg = in ? j / c.page_size : -1;
+                    if (in && pg != pg_have) {
+                        id = table[pg];
+                        pg_have = pg;
+                        if (id < 0 || id >= c.n_pages) {
+                            record_device_error(kDevErrPage);
+                            id = -1;
+                        }
+                    }
+                    const bool real = in && id >= 0 && piece_real;
+                    const int64_t off = real ? id * c.page_stride + (j - pg * c.page_size) * c.token_stride + head_off + piece * 8 : 0;
+                    cp_async16_or_zero(dst + r * kRowStep * C::kPitch, c.k + off, real);
+                    cp_async16_or_zero(dst + C::kTensorBytes + r * kRowStep * C::kPitch, c.v + off, real);
+                }
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
@@ -267,7 +310,7 @@ __global__ void __launch_bounds__(128) attention_gemv_kernel(const kvc::Cache c,
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
             base[r] = mn[r] == -INFINITY ? 0.0f : mn[r];
-            keep[r] = exp2f(m[r] - base[r]);
+            keep[r] = ex2(m[r] - base[r]);
         }
         if (__any_sync(~0u, mn[0] != m[0] || mn[1] != m[1])) {
 #pragma unroll
@@ -285,7 +328,7 @@ __global__ void __launch_bounds__(128) attention_gemv_kernel(const kvc::Cache c,
 #pragma unroll
         for (int n = 0; n < C::kKC / 8; ++n) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sc[n][e] = exp2f(sc[n][e] - base[e >> 1]);
+            for (int e = 0; e < 4; ++e) sc[n][e] = ex2(sc[n][e] - base[e >> 1]);
             l[0] += sc[n][0] + sc[n][1];
             l[1] += sc[n][2] + sc[n][3];
         }
@@ -307,10 +350,24 @@ __global__ void __launch_bounds__(128) attention_gemv_kernel(const kvc::Cache c,
             for (int d = 0; d < HD / 16; ++d) {
                 uint32_t vf[4];
                 ldsm4_t(vc + (n * 16 + ((lane >> 3) & 1) * 8 + (lane & 7)) * C::kPitch + d * 32 + (lane >> 4) * 16, vf);
+if constexpr (F32) {
+                    // The tensor core truncates as it accumulates: over thousands of keys that is
+                    // a bias of several 2^-22, so a chunk's product is summed apart, its smallest
+                    // term first, and added with a rounding.
+                    float x[4] = {}, y[4] = {};
 #pragma unroll
-                for (int w = 0; w < kTerms; ++w) {
-                    mma_bf16(o[2 * d], pf[w], vf[0], vf[1]);
-                    mma_bf16(o[2 * d + 1], pf[w], vf[2], vf[3]);
+                    for (int w = kTerms - 1; w >= 0; --w) {
+                        mma_bf16(x, pf[w], vf[0], vf[1]);
+                        mma_bf16(y, pf[w], vf[2], vf[3]);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        o[2 * d][e] += x[e];
+                        o[2 * d + 1][e] += y[e];
+                    }
+                } else {
+                    mma_bf16(o[2 * d], pf[0], vf[0], vf[1]);
+                    mma_bf16(o[2 * d + 1], pf[0], vf[2], vf[3]);
                 }
             }
         }
@@ -346,7 +403,7 @@ __global__ void __launch_bounds__(128) attention_gemv_kernel(const kvc::Cache c,
 #pragma unroll
         for (int k = 0; k < C::kWK; ++k) {
             const int w = k * WM + w0;
-            const float f = exp2f(s_m[w][rr] - base);
+            const float f = ex2(s_m[w][rr] - base);
             const float4 v = *reinterpret_cast<const float4*>(so + (w * 16 + rr) * HD + d);
             sum = fmaf(f, s_l[w][rr], sum);
             acc.x = fmaf(f, v.x, acc.x);
@@ -456,10 +513,10 @@ static int64_t longest_span(const Params& p, int tile_rows) {
     return std::max<int64_t>(span, 1);
 }
 
-template <int HD, int WM, bool F32>
+template <int HD, int WM, bool F32, bool P16>
 static int launch_gemv_tile(const kvc::Cache& c, const Params& p, const DeviceInfo& info, cudaStream_t stream) {
     using C = GemvCfg<HD, WM>;
-    auto kern = attention_gemv_kernel<HD, WM, F32>;
+    auto kern = attention_gemv_kernel<HD, WM, F32, P16>;
     static std::once_flag once[64];
     static cudaError_t prep[64];
     if (info.device < 0 || info.device >= 64) return set_error(BYBYCU_ERR_ARGS, "device %d out of range", info.device);
@@ -493,9 +550,10 @@ static int launch_gemv_tile(const kvc::Cache& c, const Params& p, const DeviceIn
 template <int HD, bool F32>
 static int launch_gemv_rows(const kvc::Cache& c, const Params& p, const DeviceInfo& info, cudaStream_t stream) {
     const int64_t rows = static_cast<int64_t>(p.max_q) * p.group;
-    if (rows <= 16) return launch_gemv_tile<HD, 1, F32>(c, p, info, stream);
-    if (rows <= 32) return launch_gemv_tile<HD, 2, F32>(c, p, info, stream);
-    return launch_gemv_tile<HD, 4, F32>(c, p, info, stream);
+    const bool p16 = c.page_size % 16 == 0;
+    if (rows <= 16) return p16 ? launch_gemv_tile<HD, 1, F32, true>(c, p, info, stream) : launch_gemv_tile<HD, 1, F32, false>(c, p, info, stream);
+    if (rows <= 32) return p16 ? launch_gemv_tile<HD, 2, F32, true>(c, p, info, stream) : launch_gemv_tile<HD, 2, F32, false>(c, p, info, stream);
+    return p16 ? launch_gemv_tile<HD, 4, F32, true>(c, p, info, stream) : launch_gemv_tile<HD, 4, F32, false>(c, p, info, stream);
 }
 
 static int launch_gemv(const kvc::Cache& c, const Params& p, bool f32, cudaStream_t stream) {
