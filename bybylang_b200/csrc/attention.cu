@@ -122,7 +122,8 @@ extern "C" int bybycu_paged_attention(const bybycu_paged_kv* kv, const bybycu_at
         return set_error(BYBYCU_ERR_SHAPE, "paged_attention: max_q=%d max_kv=%d window=%d", a->max_q, a->max_kv, a->window);
     if (!std::isfinite(a->scale) || !(a->softcap >= 0.0f) || !std::isfinite(a->softcap))
         return set_error(BYBYCU_ERR_ARGS, "paged_attention: scale %g, softcap %g", a->scale, a->softcap);
-    if (a->route != BYBYCU_ROUTE_AUTO && a->route != BYBYCU_ROUTE_SIMT && a->route != BYBYCU_ROUTE_GEMV)
+    if (a->route != BYBYCU_ROUTE_AUTO && a->route != BYBYCU_ROUTE_SIMT && a->route != BYBYCU_ROUTE_GEMV &&
+        a->route != BYBYCU_ROUTE_TC)
         return set_error(BYBYCU_ERR_ARGS, "unknown route %d", a->route);
     if (c.n_tokens == 0 || c.n_seqs == 0) return BYBYCU_OK;
     if (!a->q || !a->out) return set_error(BYBYCU_ERR_ARGS, "paged_attention: a slot is missing");
@@ -138,5 +139,12 @@ extern "C" int bybycu_paged_attention(const bybycu_paged_kv* kv, const bybycu_at
     const bool mod = a->softcap > 0.0f || a->slopes, f32 = a->out_dtype == BYBYCU_DT_F32;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (a->route == BYBYCU_ROUTE_SIMT) return attn::launch_simt(c, p, mod, f32, s);
+    const bool tc = attn::tc_attention_supports(c, p, f32);
+    if (a->route == BYBYCU_ROUTE_TC && !tc)
+        return set_error(BYBYCU_ERR_SHAPE, "paged_attention: the tensor-core route needs bf16 output, head dimension <= 128, at most "
+                                           "128 heads a group and pages of 8, 16, 32, 64 or a multiple of 128 tokens");
+    // one tensor-core tile is 128 rows
+    if (a->route == BYBYCU_ROUTE_TC || (a->route == BYBYCU_ROUTE_AUTO && tc && static_cast<int64_t>(a->max_q) * p.group > 64))
+        return attn::launch_tc_attention(c, p, mod, s);
     return attn::launch_gemv(c, p, f32, s);
 }

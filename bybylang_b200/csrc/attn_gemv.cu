@@ -51,7 +51,7 @@ __device__ __forceinline__ TileRange tile_range(const Params& p, const Seq& s, i
     r.lo = hi0 > 0 ? lo0 : 0;
     r.hi = hi1;
     r.lo_aligned = r.lo / align * align;
-    r.splits = max(1, (r.hi - r.lo_aligned + split_keys - 1) / split_keys);
+    r.splits = r.hi > r.lo_aligned ? 1 + (r.hi - r.lo_aligned - 1) / split_keys : 1;
     return r;
 }
 
@@ -120,7 +120,7 @@ __global__ void __launch_bounds__(128) attention_gemv_kernel(const kvc::Cache c,
     const TileRange range = tile_range(p, s, first_row, rows, 16, split_keys);
     if (split >= range.splits) return;
     const int seg_lo = range.lo_aligned + split * split_keys;
-    const int seg_hi = range.splits == 1 ? range.hi : min(range.hi, seg_lo + split_keys);
+    const int seg_hi = seg_lo + min(range.hi - seg_lo, split_keys);
     const int D = c.head_dim;
 
     // this thread's two rows of its warp's sixteen
@@ -425,7 +425,7 @@ if constexpr (F32) {
 // Joins the splits: one warp a row (token, head), splits in order.
 template <bool F32>
 __global__ void __launch_bounds__(128) attention_join_kernel(const kvc::Cache c, const Params p, const Partials part,
-                                                             int split_keys, int tile_rows) {
+                                                             int split_keys, int tile_rows, int align) {
     pdl_launch_dependents();
     pdl_wait();
     const int lane = threadIdx.x & 31;
@@ -437,8 +437,9 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const kvc::Cache c,
     if (b >= c.n_seqs || t < c.q_start[0]) return;
     const Seq s = load_seq(c, p, b);
     if (t - s.q0 >= s.rows) return;
+    // the tile that the row was in: key range and splits as that kernel had them
     const int first_row = ((t - s.q0) * p.group + h % p.group) / tile_rows * tile_rows;
-    const TileRange range = tile_range(p, s, first_row, min(tile_rows, s.rows * p.group - first_row), 16, split_keys);
+    const TileRange range = tile_range(p, s, first_row, min(tile_rows, s.rows * p.group - first_row), align, split_keys);
     if (range.splits == 1) return;   // written by the first kernel
     float mx = -INFINITY;
     for (int k = lane; k < range.splits; k += 32) mx = fmaxf(mx, part.ml[k * part.rows + row].x);
@@ -477,12 +478,12 @@ static cudaLaunchConfig_t pdl_config(dim3 grid, int threads, size_t smem, cudaSt
     return cfg;
 }
 
-static int launch_join(const kvc::Cache& c, const Params& p, const Partials& part, int split_keys, int tile_rows, bool f32,
-                       cudaStream_t stream) {
+static int launch_join(const kvc::Cache& c, const Params& p, const Partials& part, int split_keys, int tile_rows,
+                       int align, bool f32, cudaStream_t stream) {
     cudaLaunchAttribute attr[1];
     const cudaLaunchConfig_t cfg = pdl_config(dim3(static_cast<unsigned>(ceil_div(part.rows, 4))), 128, 0, stream, attr);
     BYBYCU_CUDA_TRY(cudaLaunchKernelEx(&cfg, f32 ? attention_join_kernel<true> : attention_join_kernel<false>, c, p, part,
-                                       split_keys, tile_rows));
+                                       split_keys, tile_rows, align));
     return BYBYCU_OK;
 }
 
@@ -544,7 +545,7 @@ static int launch_gemv_tile(const kvc::Cache& c, const Params& p, const DeviceIn
     const cudaLaunchConfig_t cfg = pdl_config(dim3(static_cast<unsigned>(splits), static_cast<unsigned>(row_tiles * c.kv_heads),
                                                    static_cast<unsigned>(c.n_seqs)), 128, C::kSmem, stream, attr);
     BYBYCU_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, c, p, part, split_keys, row_tiles));
-    return splits > 1 ? launch_join(c, p, part, split_keys, 16 * WM, F32, stream) : BYBYCU_OK;
+    return splits > 1 ? launch_join(c, p, part, split_keys, 16 * WM, 16, F32, stream) : BYBYCU_OK;
 }
 
 template <int HD, bool F32>

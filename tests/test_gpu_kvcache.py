@@ -25,10 +25,16 @@ F32_TOL = 6e-5
 BF16_TOL = 2.0 ** -7 + F32_TOL
 
 
+def tc_runs(bt, out_dtype):
+    return bt.dim <= 128 and out_dtype == torch.bfloat16 and bt.page % 8 == 0 and (128 % bt.page == 0 or bt.page % 128 == 0)
+
+
 def check(bt, route, out_dtype=torch.float32, **mods):
     kw = dict(mods)
     if kw.get("slopes") is not None:
         kw["slopes"] = kw["slopes"].to(DEV)
+    if route == TC and not tc_runs(bt, out_dtype):
+        pytest.skip("no tensor-core form of this shape")
     prefix = kw.pop("prefix", None)
     if prefix is not None:
         kw["prefix_lens"] = torch.tensor(prefix, dtype=torch.int32, device=DEV)
@@ -48,7 +54,7 @@ DECODE = [(1, n) for n in (1, 2, 15, 16, 17, 63, 64, 65, 127, 128, 129, 500, 0)]
 
 
 @pytest.mark.parametrize("out_dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("route", [AUTO, GEMV, SIMT])
+@pytest.mark.parametrize("route", [AUTO, GEMV, SIMT, TC])
 @pytest.mark.parametrize("dim,page,heads,kv_heads", [(64, 16, 8, 2), (128, 64, 4, 4), (128, 16, 8, 1), (8, 1, 3, 1),
                                                      (80, 7, 6, 2), (96, 48, 5, 5), (256, 128, 2, 1), (40, 256, 4, 2)])
 @pytest.mark.parametrize("lens", [RAGGED, DECODE], ids=["ragged", "decode"])
@@ -66,7 +72,7 @@ MODS = [dict(softcap=5.0), dict(softcap=30.0, window=40), dict(window=1), dict(w
         dict(slopes=True), dict(slopes=True, softcap=20.0, prefix=[37] * 8, window=100), dict(scale=0.0), dict(scale=-0.3)]
 
 
-@pytest.mark.parametrize("route", [AUTO, GEMV, SIMT])
+@pytest.mark.parametrize("route", [AUTO, GEMV, SIMT, TC])
 @pytest.mark.parametrize("dim,page,heads,kv_heads", [(64, 16, 8, 2), (128, 64, 4, 4), (80, 7, 6, 2), (128, 32, 24, 1)])
 @pytest.mark.parametrize("mods", MODS, ids=lambda m: "-".join(m))
 def test_attention_masks_and_scores(mods, dim, page, heads, kv_heads, route):
@@ -74,14 +80,15 @@ def test_attention_masks_and_scores(mods, dim, page, heads, kv_heads, route):
     if mods.get("slopes"):
         mods["slopes"] = 2.0 ** (-8.0 * torch.arange(1, heads + 1) / heads)
     bt = Batch(RAGGED, page=page, heads=heads, kv_heads=kv_heads, dim=dim, seed=3)
-    check(bt, route, **mods)
+    dtype = torch.bfloat16 if route == TC else torch.float32
+    check(bt, route, dtype, **mods)
     one = dict(mods)
     if one.get("prefix"):
         one["prefix"] = (one["prefix"] * 2)[:len(DECODE)]
-    check(Batch(DECODE, page=page, heads=heads, kv_heads=kv_heads, dim=dim, seed=4), route, **one)
+    check(Batch(DECODE, page=page, heads=heads, kv_heads=kv_heads, dim=dim, seed=4), route, dtype, **one)
 
 
-@pytest.mark.parametrize("route", [AUTO, GEMV, SIMT])
+@pytest.mark.parametrize("route", [AUTO, GEMV, SIMT, TC])
 @pytest.mark.parametrize("lens", [[(1, 400), (1, 90)], [(40, 400), (200, 390)]], ids=["decode", "chunk"])
 def test_attention_pages_before_the_window_are_gone(lens, route):
     """A freed page (-1 in the table, its memory someone else's NaN) before the window is not touched."""
@@ -92,19 +99,39 @@ def test_attention_pages_before_the_window_are_gone(lens, route):
             bt.k[first] = float("nan")
             bt.v[first] = float("nan")
             bt.table[b, pg] = -1
-    check(bt, route, window=50)
+    check(bt, route, torch.bfloat16 if route == TC else torch.float32, window=50)
 
 
-@pytest.mark.parametrize("route", [AUTO, GEMV, SIMT])
+@pytest.mark.parametrize("route", [AUTO, GEMV, SIMT, TC])
 def test_attention_large_scores(route):
     """Scores in the hundreds: the running maximum carries the sums, whatever order the keys come in."""
     bt = Batch([(1, 700), (70, 700)], page=64, heads=4, kv_heads=1, dim=64, seed=5, spread=40.0)
     # the score error scales with the scores: 64 * 2^-24 * sum|qk| * scale <= 2e-3 here
-    out = torch.empty((bt.tokens, 4, 64), dtype=torch.float32, device=DEV)
+    out = torch.empty((bt.tokens, 4, 64), dtype=torch.bfloat16 if route == TC else torch.float32, device=DEV)
     kv.paged_attention(bt.q, *bt.args(), max_q=bt.max_q, max_kv=bt.max_kv, out=out, route=route)
     want = attention64(bt)
     assert torch.isfinite(out).all()
-    assert float((out.cpu().double() - want).abs().max()) <= 2e-3 * max(float(v.abs().max()) for v in bt.values)
+    assert float((out.cpu().double() - want).abs().max()) <= (2e-3 + (2.0 ** -7 if route == TC else 0.0)) * max(float(v.abs().max()) for v in bt.values)
+
+
+@pytest.mark.parametrize("route", [AUTO, GEMV, TC])
+@pytest.mark.parametrize("dim,page,heads,kv_heads", [(64, 16, 12, 4), (128, 128, 4, 4), (96, 32, 7, 1), (128, 8, 32, 1)])
+@pytest.mark.parametrize("mods", [dict(), dict(window=200), dict(softcap=20.0, prefix=[300, 700, 0])], ids=["plain", "window", "capped"])
+def test_attention_prompts(mods, dim, page, heads, kv_heads, route):
+    """Many tiles of rows and blocks of keys: chunks that start inside a cache and end anywhere."""
+    bt = Batch([(300, 300), (257, 900), (33, 1111)], page=page, heads=heads, kv_heads=kv_heads, dim=dim, seed=11)
+    check(bt, route, torch.bfloat16, **mods)
+
+
+@pytest.mark.parametrize("out_dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("route", [AUTO, GEMV, TC])
+def test_attention_split_caches(route, out_dtype):
+    """Few rows over a long cache: the keys split across the grid and joined."""
+    bt = Batch([(40, 5000)], page=64, heads=8, kv_heads=2, dim=128, seed=12)
+    check(bt, route, out_dtype)
+    check(bt, route, out_dtype, window=3000)
+    bt = Batch([(1, 9000), (2, 700), (1, 3)], page=16, heads=8, kv_heads=1, dim=64, seed=13)
+    check(bt, route, out_dtype)
 
 
 def test_attention_bad_metadata_is_recorded_not_followed():
