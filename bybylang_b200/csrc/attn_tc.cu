@@ -91,6 +91,26 @@ __device__ __forceinline__ void commit(uint64_t* bar) {
                  ::"r"(smem_u32(bar)) : "memory");
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+        "fma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+
 template <int HD, bool MOD>
 __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_constant__ Maps maps, const kvc::Cache c,
                                                                    const Params p, const Partials part, int split_keys,
@@ -157,6 +177,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
     tc::tc_fence_after();
     const uint32_t tmem = *tmem_slot;
 
+    // A score row is 128 registers: the softmax groups take them from the other four warps
+    // (256 * 216 + 128 * 72 = 384 * 168, what the launch holds).
+    if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp == 8) {
         // ----------------------------------------------------------------- loads
         if (n_all > 0) {
@@ -288,8 +312,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
         if (!ok && n_all > 0) *s_abort = 1;
         commit(done);
         __all_sync(~0u, tc::wait_bar(done, 0, kDevErrMmaWait));
-    } else if (warp < 8) {
+    }
+    } else {
         // ----------------------------------------------------------------- softmax, one row a thread
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         const int i = warp >> 2, r = threadIdx.x & 127;
         const int my_rows = min(tile_rows, rows - i * tile_rows);
         const int row = first_row + i * tile_rows + r;
@@ -329,9 +355,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
             float mx[4];
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                mx[q] = __uint_as_float(sc[q][0]);
+                mx[q] = fmaxf(__uint_as_float(sc[q][0]), __uint_as_float(sc[q][1]));
 #pragma unroll
-                for (int e = 1; e < 32; ++e) mx[q] = fmaxf(mx[q], __uint_as_float(sc[q][e]));
+                for (int e = 2; e < 32; e += 2) mx[q] = max3(mx[q], __uint_as_float(sc[q][e]), __uint_as_float(sc[q][e + 1]));
             }
             const float mn = fmaxf(m, unit * fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
             if (__any_sync(~0u, mn > m + 8.0f)) {
@@ -352,21 +378,22 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
                 }
             }
             const float off = m == -INFINITY ? 0.0f : m;
+            const float2 unit2 = make_float2(unit, unit), off2 = make_float2(-off, -off);
+            float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 uint32_t pk[16];
-                float sum[2] = {0.0f, 0.0f};
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    const float x = ex2(fmaf(__uint_as_float(sc[q][2 * e]), unit, -off));
-                    const float y = ex2(fmaf(__uint_as_float(sc[q][2 * e + 1]), unit, -off));
-                    sum[0] += x;
-                    sum[1] += y;
-                    pk[e] = pack_bf16(x, y);
+                    float2 x = fma2(make_float2(__uint_as_float(sc[q][2 * e]), __uint_as_float(sc[q][2 * e + 1])), unit2, off2);
+                    x.x = ex2(x.x);
+                    x.y = ex2(x.y);
+                    sum = add2(sum, x);
+                    pk[e] = pack_bf16(x.x, x.y);
                 }
-                l += sum[0] + sum[1];
                 tc::tmem_st16(ts + 16 * q, pk);
             }
+            l += sum.x + sum.y;
             tc::tc_wait_st();
             tc::tc_fence_before();
             __syncwarp();
