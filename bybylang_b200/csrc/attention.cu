@@ -135,7 +135,7 @@ extern "C" int bybycu_paged_attention(const bybycu_paged_kv* kv, const bybycu_at
     const attn::Params p{static_cast<const __nv_bfloat16*>(a->q), a->out, a->q_token_stride, a->q_head_stride,
                          a->out_token_stride, a->out_head_stride, a->slopes, a->prefix_lens, a->q_heads,
                          a->q_heads / c.kv_heads, a->max_q, a->max_kv, a->window, a->scale * attn::kLog2e, a->softcap,
-                         a->softcap > 0.0f ? a->scale / a->softcap : 0.0f};
+                         a->softcap > 0.0f ? 2.0f * attn::kLog2e * (a->scale / a->softcap) : 0.0f, a->softcap * attn::kLog2e};
     const bool mod = a->softcap > 0.0f || a->slopes, f32 = a->out_dtype == BYBYCU_DT_F32;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (a->route == BYBYCU_ROUTE_SIMT) return attn::launch_simt(c, p, mod, f32, s);

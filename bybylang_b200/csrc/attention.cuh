@@ -16,7 +16,7 @@ struct Params {
     const float* slopes;
     const int32_t* prefix;
     int32_t q_heads, group, max_q, max_kv, window;   // group: query heads a kv head
-    float scale_log2, cap, scale_over_cap;           // scale * log2(e); softcap; scale / softcap
+    float scale_log2, cap, cap_in, cap_out;          // scale * log2(e); softcap; 2 log2(e) scale / softcap; softcap * log2(e)
 };
 
 // One sequence of the batch as a kernel reads it.  rows and kv are what may be touched: never past
@@ -53,21 +53,24 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
-// The score of a pair in units of log2: raw = q . k.
-//   MOD: a tanh cap and / or distance slopes.  tanh(y) = 1 - 2 / (1 + e^2y) with the hardware's
-//   exponential and reciprocal: its absolute error is a few 2^-24, times the cap.
+// cap * tanh(y) of two scores in units of log2, y = raw * scale / cap: tanh(y) = 1 - 2 / (1 + e^2y)
+// with the hardware's exponential and one reciprocal for both.  The absolute error is a few
+// 2^-24 times the cap.  2 y log2(e) is held below 60, where tanh is 1 in fp32, so that the
+// product of the two denominators stays finite.
+__device__ __forceinline__ float2 capped_log2(const Params& p, float raw0, float raw1) {
+    const float a = 1.0f + ex2(fminf(raw0 * p.cap_in, 60.0f)), b = 1.0f + ex2(fminf(raw1 * p.cap_in, 60.0f));
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(a * b));
+    return make_float2(fmaf(-2.0f * p.cap_out, r * b, p.cap_out), fmaf(-2.0f * p.cap_out, r * a, p.cap_out));
+}
+
+// The score of a pair in units of log2: raw = q . k, MOD: a cap and / or distance slopes.
 template <bool MOD>
 __device__ __forceinline__ float score_log2(const Params& p, float raw, float slope_log2, int distance) {
     if constexpr (!MOD) {
         return raw * p.scale_log2;
     } else {
-        float s;
-        if (p.cap > 0.0f) {
-            const float y = raw * p.scale_over_cap;
-            s = p.cap * kLog2e * (1.0f - __fdividef(2.0f, 1.0f + ex2(2.0f * kLog2e * y)));
-        } else {
-            s = raw * p.scale_log2;
-        }
+        const float s = p.cap > 0.0f ? capped_log2(p, raw, 0.0f).x : raw * p.scale_log2;
         return s - slope_log2 * static_cast<float>(distance < 0 ? -distance : distance);
     }
 }

@@ -341,10 +341,25 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
             for (int q = 0; q < 4; ++q) tc::tmem_ld32(ts + 32 * q, sc[q]);
             tc::tc_wait_ld();
             const int t0 = seg_lo + j * kKeys;
-            if (MOD) {
+            if constexpr (MOD) {
+                if (p.cap > 0.0f) {
 #pragma unroll
-                for (int e = 0; e < kKeys; ++e)
-                    sc[e / 32][e % 32] = __float_as_uint(score_log2<true>(p, __uint_as_float(sc[e / 32][e % 32]), slope, pos - (t0 + e)));
+                    for (int e = 0; e < kKeys; e += 2) {
+                        uint32_t &u0 = sc[e / 32][e % 32], &u1 = sc[e / 32][e % 32 + 1];
+                        const float2 t = capped_log2(p, __uint_as_float(u0), __uint_as_float(u1));
+                        u0 = __float_as_uint(t.x);
+                        u1 = __float_as_uint(t.y);
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < kKeys; ++e) sc[e / 32][e % 32] = __float_as_uint(__uint_as_float(sc[e / 32][e % 32]) * p.scale_log2);
+                }
+                if (p.slopes) {
+                    const float dist = static_cast<float>(pos - t0);
+#pragma unroll
+                    for (int e = 0; e < kKeys; ++e)
+                        sc[e / 32][e % 32] = __float_as_uint(fmaf(-slope, fabsf(dist - static_cast<float>(e)), __uint_as_float(sc[e / 32][e % 32])));
+                }
             }
             if (__any_sync(~0u, t0 < row_lo || t0 + kKeys > row_hi)) {
                 const int lo = row_lo - t0, hi = row_hi - t0;
