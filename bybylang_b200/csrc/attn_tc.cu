@@ -4,15 +4,17 @@
 // A CTA (one per SM) takes two tiles of up to 128 query rows of one kv head - row r is token
 // r / G, head r % G, so the G heads of a group share every key they read - and walks the keys in
 // blocks of 128:
-//   warps 0-3, 4-7   one softmax group per query tile, one row a thread
-//   warp 8           brings Q and the K and V blocks in by TMA, page by page through the table
-//   warp 9           issues the MMAs: S = Q K^T (both from shared memory) into tensor memory,
+//   warps 0-7, 8-15  one softmax group per query tile: two threads a row, 64 keys each
+//   warp 16          brings Q and the K and V blocks in by TMA, page by page through the table
+//   warp 17          issues the MMAs: S = Q K^T (both from shared memory) into tensor memory,
 //                    O += P V with P from tensor memory (bf16, over the scores it came from)
 //                    and V as it lies in its pages (N-major)
 // While the tensor core works on one tile's O += P V and next S, the other tile's group is at its
 // exponentials: at 128 dimensions a block's two products take the tensor core about as long
 // (2 * 128^3 multiplies at 4096 a cycle) as its 128^2 exponentials take the SM's special-function
-// units (16 a cycle), so neither may wait for the other.
+// units (16 a cycle), so neither may wait for the other.  One thread a row took 4800 cycles a pair
+// of blocks (tensor core and special-function units 37% busy each, ncu): the chain scores - maximum
+// - exponentials - probabilities of 128 keys in one thread was longer than the other tile's MMAs.
 //
 //   * The running maximum is only followed when it grew by more than 2^8: probabilities then stay
 //     below 2^8, with the same relative rounding in bf16 and sums in fp32, and the accumulators in
@@ -33,7 +35,9 @@ namespace bybycu {
 namespace attn {
 namespace tcore {
 
-constexpr int kThreads = 384;
+constexpr int kThreads = 640;
+constexpr int kLoadWarp = 16, kMmaWarp = 17;
+constexpr int kHalf = 64;       // keys of a softmax thread
 constexpr int kRows = 128;      // query rows of a tile (MMA M)
 constexpr int kKeys = 128;      // keys of a block
 constexpr uint32_t kTmemCols = 512;
@@ -43,13 +47,14 @@ struct Cfg {
     static constexpr int kHalves = HD / 64;                              // 128-byte swizzled boxes a row
     static constexpr uint32_t kQTile = kRows * HD * 2;
     static constexpr uint32_t kBlock = kKeys * HD * 2;                   // one K or V block
-    static constexpr int kStages = HD == 128 ? 5 : 8;
+    static constexpr int kStages = HD == 128 ? 4 : 8;
     static constexpr uint32_t kOffRing = 2 * kQTile;
     static constexpr uint32_t kOffBar = kOffRing + kStages * kBlock;
     // barriers: q; full, empty [stages]; s_full, p_full [2]; done
     static constexpr uint32_t kNumBars = 1 + 2 * kStages + 4 + 1;
     static constexpr uint32_t kOffSlot = kOffBar + kNumBars * 8;
-    static constexpr uint32_t kSmem = kOffSlot + 8 + 1024;               // + alignment slack
+    static constexpr uint32_t kOffRow = kOffSlot + 8;                    // a float per thread of the softmax groups
+    static constexpr uint32_t kSmem = kOffRow + 512 * 4 + 1024;          // + alignment slack
     static_assert(kSmem <= 227 * 1024 && kSmem > 114 * 1024, "one CTA per SM");
     // instruction descriptors of kind::f16: D fp32, A and B bf16, M = 128
     static constexpr uint32_t kBase = (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(kRows >> 4) << 24);
@@ -74,21 +79,64 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
                  ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3) : "memory");
 }
 
-// The MMA warp stays converged; elect.sync picks the lane that issues.
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred e, p;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+// The MMA warp stays converged; elect.sync picks the lane that issues.  Four products at a time
+// (an instruction of its own to elect for each would cost as much as the issue).
+__device__ __forceinline__ void mma_ss4(uint32_t d, const uint64_t (&a)[4], const uint64_t (&b)[4], uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred e, p, q;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %2, 0;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+                 "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %3, %7, %1, p;\n\t"
+                 "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %4, %8, %1, q;\n\t"
+                 "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %5, %9, %1, q;\n\t"
+                 "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %6, %10, %1, q;\n\t}"
+                 ::"r"(d), "r"(idesc), "r"(accumulate), "l"(a[0]), "l"(a[1]), "l"(a[2]), "l"(a[3]), "l"(b[0]), "l"(b[1]), "l"(b[2]), "l"(b[3])
+                 : "memory");
 }
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile("{\n\t.reg .pred e, p;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
                  "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
                  ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
+// The same from tensor memory: A 8 columns (16 keys) further each, B 2048 bytes.
+__device__ __forceinline__ void mma_ts4(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred e, p, q;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %2, 0;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+                 "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%3], %7, %1, p;\n\t"
+                 "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%4], %8, %1, q;\n\t"
+                 "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%5], %9, %1, q;\n\t"
+                 "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%6], %10, %1, q;\n\t}"
+                 ::"r"(d), "r"(idesc), "r"(accumulate), "r"(a), "r"(a + 8), "r"(a + 16), "r"(a + 24), "l"(b), "l"(b + 128), "l"(b + 256),
+                 "l"(b + 384)
+                 : "memory");
+}
 __device__ __forceinline__ void commit(uint64_t* bar) {
     asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
                  "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
                  ::"r"(smem_u32(bar)) : "memory");
+}
+
+// Bounded wait that also ends when another warp of the CTA has given up (without reading its
+// flag where the phase is complete already: a shared-memory read costs the chain of waits some
+// 100 cycles while the tensor core streams its operands).
+__device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, volatile int* abort, uint32_t err) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const uint64_t t0 = globaltimer_ns();
+    for (;;) {
+#pragma unroll 1
+        for (int i = 0; i < 64; ++i)
+            if (mbar_try_wait(bar, parity)) return true;
+        if (*abort) return false;
+        if (globaltimer_ns() - t0 > kWaitLimitNs) {
+            record_device_error(err);
+            *abort = 1;
+            return false;
+        }
+    }
+}
+
+// Whether any of the 256 threads of a softmax group says so; their barrier.
+__device__ __forceinline__ bool group_any(uint32_t id, bool mine) {
+    uint32_t any;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, %2, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                 : "=r"(any) : "r"(static_cast<uint32_t>(mine)), "r"(id) : "memory");
+    return any != 0;
 }
 
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -161,13 +209,13 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&s_full[i], 1);
-            mbar_init(&p_full[i], 4);
+            mbar_init(&p_full[i], 8);
         }
         mbar_init(done, 1);
         *s_abort = 0;
         fence_mbar_init();
     }
-    if (warp == 9) {
+    if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
                      ::"r"(smem_u32(const_cast<uint32_t*>(tmem_slot))), "r"(kTmemCols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -177,146 +225,148 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
     tc::tc_fence_after();
     const uint32_t tmem = *tmem_slot;
 
-    // A score row is 128 registers: the softmax groups take them from the other four warps
-    // (256 * 216 + 128 * 72 = 384 * 168, what the launch holds).
-    if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-    if (warp == 8) {
-        // ----------------------------------------------------------------- loads
-        if (n_all > 0) {
-            if (lane == 0) {
-                const int tokens = tile_rows / p.group;
-                const uint32_t bytes = static_cast<uint32_t>(tile_rows) * 128u * C::kHalves;
-                mbar_arrive_expect_tx(q_full, n_blocks[1] > 0 ? 2 * bytes : bytes);
-                for (int i = 0; i < (n_blocks[1] > 0 ? 2 : 1); ++i)
-                    for (int h = 0; h < C::kHalves; ++h)
-                        tma_load_3d(base + i * C::kQTile + h * kRows * 128, &maps.q, q_full, h * 64, kvh * p.group,
-                                    s.q0 + first_row / p.group + i * tokens);
-            }
-            // lane l looks after the block's slots [l * box, l * box + box)
-            const int boxes = kKeys / box_slots;
-            const int32_t* table = c.page_table + b * c.table_stride;
-            auto look_up = [&](int j, int* slot) {
-                const int key = seg_lo + j * kKeys + lane * box_slots;
-                if (lane >= boxes || key >= seg_hi || key + box_slots <= range.lo) return -1;
-                const int pg = key / c.page_size;
-                *slot = key - pg * c.page_size;
-                return table[pg];
-            };
-            int slot = 0, next_slot = 0, issued = 0;
-            int next_id = look_up(0, &next_slot);
-            bool ok = true;
-            for (int j = 0; j < n_all && ok; ++j) {
-                const int key = seg_lo + j * kKeys + lane * box_slots;
-                const bool mine = lane < boxes && key < seg_hi && key + box_slots > range.lo;
-                int id = next_id;
-                slot = next_slot;
-                if (j + 1 < n_all) next_id = look_up(j + 1, &next_slot);
-                if (mine && (id < 0 || id >= c.n_pages)) {
-                    record_device_error(kDevErrPage);
-                    id = c.n_pages;   // past the tensor: the copy fills zeros
-                }
-                const uint32_t n_boxes = __popc(__ballot_sync(~0u, mine));
-                for (int kv = 0; kv < 2; ++kv, ++issued) {
-                    const int st = issued % C::kStages, r = issued / C::kStages;
-                    if (r > 0 && !__all_sync(~0u, tc::wait_bar(&empty[st], (r - 1) & 1, kDevErrEmptyWait))) ok = false;
-                    if (__any_sync(~0u, *s_abort != 0)) ok = false;
-                    if (!ok) break;
-                    if (lane == 0) mbar_arrive_expect_tx(&full[st], n_boxes * static_cast<uint32_t>(box_slots) * 128u * C::kHalves);
-                    __syncwarp();
-                    if (mine)
+    // The softmax groups take registers from the other four warps (512 * 104 + 128 * 64 = 640 * 96,
+    // what the launch holds).
+    if (warp >= kLoadWarp) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        if (warp == kLoadWarp) {
+            // ----------------------------------------------------------------- loads
+            if (n_all > 0) {
+                if (lane == 0) {
+                    const int tokens = tile_rows / p.group;
+                    const uint32_t bytes = static_cast<uint32_t>(tile_rows) * 128u * C::kHalves;
+                    mbar_arrive_expect_tx(q_full, n_blocks[1] > 0 ? 2 * bytes : bytes);
+                    for (int i = 0; i < (n_blocks[1] > 0 ? 2 : 1); ++i)
                         for (int h = 0; h < C::kHalves; ++h)
-                            tma_load_4d(base + C::kOffRing + st * C::kBlock + h * kKeys * 128 + lane * box_slots * 128,
-                                        kv ? &maps.v : &maps.k, &full[st], h * 64, slot, kvh, id);
+                            tma_load_3d(base + i * C::kQTile + h * kRows * 128, &maps.q, q_full, h * 64, kvh * p.group,
+                                        s.q0 + first_row / p.group + i * tokens);
                 }
-            }
-            if (!ok) *s_abort = 1;
-            // leave no copy in flight
-            if (!tc::wait_bar(q_full, 0, kDevErrDrainWait)) *s_abort = 1;
-            for (int it = max(0, issued - C::kStages); it < issued; ++it)
-                if (!tc::wait_bar(&full[it % C::kStages], (it / C::kStages) & 1, kDevErrDrainWait)) break;
-        }
-    } else if (warp == 9) {
-        // ----------------------------------------------------------------- MMAs
-        bool ok = n_all > 0 && __all_sync(~0u, tc::wait_bar(q_full, 0, kDevErrFullWait));
-        auto wait_stage = [&](int it) { return __all_sync(~0u, tc::wait_bar(&full[it % C::kStages], (it / C::kStages) & 1, kDevErrFullWait)); };
-        auto issue_s = [&](int i, int it) {
-            const uint64_t q = tc::sw128_desc(base + i * C::kQTile);
-            const uint64_t k = tc::sw128_desc(base + C::kOffRing + it % C::kStages * C::kBlock);
-#pragma unroll
-            for (int k16 = 0; k16 < HD / 16; ++k16) {
-                // 16 dimensions are 32 bytes inside a swizzled row; 64 are the next box
-                const uint64_t off = static_cast<uint64_t>((k16 >> 2) * (kRows * 128 >> 4) + (k16 & 3) * 2);
-                mma_ss(tmem + i * kKeys, q + off, k + off, C::kIdescS, k16 != 0);
-            }
-        };
-        if (ok) {
-            ok = wait_stage(0);
-            if (ok) {
-                tc::tc_fence_after();
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-                    if (n_blocks[i] > 0) {
-                        issue_s(i, 0);
-                        commit(&s_full[i]);
+                // lane l looks after the block's slots [l * box, l * box + box)
+                const int boxes = kKeys / box_slots;
+                const int32_t* table = c.page_table + b * c.table_stride;
+                auto look_up = [&](int j, int* slot) {
+                    const int key = seg_lo + j * kKeys + lane * box_slots;
+                    if (lane >= boxes || key >= seg_hi || key + box_slots <= range.lo) return -1;
+                    const int pg = key / c.page_size;
+                    *slot = key - pg * c.page_size;
+                    return table[pg];
+                };
+                int slot = 0, next_slot = 0, issued = 0;
+                int next_id = look_up(0, &next_slot);
+                bool ok = true;
+                for (int j = 0; j < n_all && ok; ++j) {
+                    const int key = seg_lo + j * kKeys + lane * box_slots;
+                    const bool mine = lane < boxes && key < seg_hi && key + box_slots > range.lo;
+                    int id = next_id;
+                    slot = next_slot;
+                    if (j + 1 < n_all) next_id = look_up(j + 1, &next_slot);
+                    if (mine && (id < 0 || id >= c.n_pages)) {
+                        record_device_error(kDevErrPage);
+                        id = c.n_pages;   // past the tensor: the copy fills zeros
                     }
-                commit(&empty[0]);
-            }
-        }
-        for (int j = 0; j < n_all && ok; ++j) {
-            const int v_it = 2 * j + 1, k_it = 2 * j + 2;
-            // the 16-key steps that hold a key which some row sees
-            const int t0 = seg_lo + j * kKeys;
-            const int lo = max(0, range.lo - t0), hi = min(kKeys, seg_hi - t0);
-            const int step0 = lo / 16, step1 = (hi + 15) / 16;
-            const uint32_t v_smem = base + C::kOffRing + v_it % C::kStages * C::kBlock;
-            bool have_v = false, have_k = false;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                if (j >= n_blocks[i] || !ok) continue;
-                ok = __all_sync(~0u, tc::wait_bar(&p_full[i], j & 1, kDevErrMmaWait));
-                if (ok && !have_v) {
-                    ok = have_v = wait_stage(v_it);
-                    if (ok && (lo > step0 * 16 || hi < step1 * 16)) {
-                        // V rows of the outer steps that belong to no visible key
-                        const int n0 = lo - step0 * 16, n1 = step1 * 16 - hi, per = HD / 8;
-                        for (int e = lane; e < (n0 + n1) * per; e += 32) {
-                            const int r = e / per < n0 ? step0 * 16 + e / per : hi + e / per - n0, d = e % per;
-                            const uint32_t at = v_smem + (d >> 3) * (kKeys * 128) + r * 128 + ((d & 7) ^ (r & 7)) * 16;
-                            sts_v4(at, 0.0f, 0.0f, 0.0f, 0.0f);
-                        }
-                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    const uint32_t n_boxes = __popc(__ballot_sync(~0u, mine));
+                    for (int kv = 0; kv < 2; ++kv, ++issued) {
+                        const int st = issued % C::kStages, r = issued / C::kStages;
+                        if (r > 0) ok = __all_sync(~0u, wait_or_abort(&empty[st], (r - 1) & 1, s_abort, kDevErrEmptyWait));
+                        if (!ok) break;
+                        if (lane == 0) mbar_arrive_expect_tx(&full[st], n_boxes * static_cast<uint32_t>(box_slots) * 128u * C::kHalves);
                         __syncwarp();
+                        if (mine)
+                            for (int h = 0; h < C::kHalves; ++h)
+                                tma_load_4d(base + C::kOffRing + st * C::kBlock + h * kKeys * 128 + lane * box_slots * 128,
+                                            kv ? &maps.v : &maps.k, &full[st], h * 64, slot, kvh, id);
                     }
                 }
+                if (!ok) *s_abort = 1;
+                // leave no copy in flight
+                if (!tc::wait_bar(q_full, 0, kDevErrDrainWait)) *s_abort = 1;
+                for (int it = max(0, issued - C::kStages); it < issued; ++it)
+                    if (!tc::wait_bar(&full[it % C::kStages], (it / C::kStages) & 1, kDevErrDrainWait)) break;
+            }
+        } else if (warp == kMmaWarp) {
+            // ----------------------------------------------------------------- MMAs
+            bool ok = n_all > 0 && __all_sync(~0u, wait_or_abort(q_full, 0, s_abort, kDevErrFullWait));
+            auto wait_stage = [&](int it) { return __all_sync(~0u, wait_or_abort(&full[it % C::kStages], (it / C::kStages) & 1, s_abort, kDevErrFullWait)); };
+            auto issue_s = [&](int i, int it) {
+                const uint64_t q = tc::sw128_desc(base + i * C::kQTile);
+                const uint64_t kk = tc::sw128_desc(base + C::kOffRing + it % C::kStages * C::kBlock);
+#pragma unroll
+                for (int h = 0; h < C::kHalves; ++h) {
+                    uint64_t qd[4], kd[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {   // 16 dimensions are 32 bytes inside a swizzled row, 64 the next box
+                        qd[k] = q + static_cast<uint64_t>(h * (kRows * 128 >> 4) + k * 2);
+                        kd[k] = kk + static_cast<uint64_t>(h * (kKeys * 128 >> 4) + k * 2);
+                    }
+                    mma_ss4(tmem + i * kKeys, qd, kd, C::kIdescS, h != 0);
+                }
+            };
+            if (ok) {
+                ok = wait_stage(0);
+                if (ok) {
+                    tc::tc_fence_after();
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+                        if (n_blocks[i] > 0) {
+                            issue_s(i, 0);
+                            commit(&s_full[i]);
+                        }
+                    commit(&empty[0]);
+                }
+            }
+            for (int j = 0; j < n_all && ok; ++j) {
+                const int v_it = 2 * j + 1, k_it = 2 * j + 2;
+                // the 16-key steps that hold a key which some row sees
+                const int t0 = seg_lo + j * kKeys;
+                const int lo = max(0, range.lo - t0), hi = min(kKeys, seg_hi - t0);
+                const int step0 = lo / 16, step1 = (hi + 15) / 16;
+                const uint32_t v_smem = base + C::kOffRing + v_it % C::kStages * C::kBlock;
+                // the loads first, so that nothing but the issue follows the probabilities
+                ok = wait_stage(v_it) && (j + 1 >= n_all || wait_stage(k_it));
                 if (!ok) break;
-                tc::tc_fence_after();
+                if (lo > step0 * 16 || hi < step1 * 16) {
+                    // V rows of the outer steps that belong to no visible key
+                    const int n0 = lo - step0 * 16, n1 = step1 * 16 - hi, per = HD / 8;
+                    for (int e = lane; e < (n0 + n1) * per; e += 32) {
+                        const int r = e / per < n0 ? step0 * 16 + e / per : hi + e / per - n0, d = e % per;
+                        const uint32_t at = v_smem + (d >> 3) * (kKeys * 128) + r * 128 + ((d & 7) ^ (r & 7)) * 16;
+                        sts_v4(at, 0.0f, 0.0f, 0.0f, 0.0f);
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                }
                 // V is [key][dim]: N-major, 64-dim boxes kKeys * 128 bytes apart, 8-key groups 1024
                 const uint64_t vd = (static_cast<uint64_t>((v_smem >> 4) & 0x3FFFu)) |
                                     (static_cast<uint64_t>(kKeys * 128 >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
-                for (int st = step0; st < step1; ++st)
-                    mma_ts(tmem + C::kTmemO + i * HD, tmem + i * kKeys + st * 8, vd + st * (2048 >> 4), C::kIdescO,
-                           j > 0 || st > step0);
-                if (j + 1 < n_blocks[i]) {
-                    if (!have_k) ok = have_k = wait_stage(k_it);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    if (j >= n_blocks[i]) continue;
+                    ok = __all_sync(~0u, wait_or_abort(&p_full[i], j & 1, s_abort, kDevErrMmaWait));
                     if (!ok) break;
                     tc::tc_fence_after();
-                    issue_s(i, k_it);
+                    const uint32_t o = tmem + C::kTmemO + i * HD, pr = tmem + i * kKeys;
+                    if (step0 == 0 && step1 == kKeys / 16) {
+                        mma_ts4(o, pr, vd, C::kIdescO, j > 0);
+                        mma_ts4(o, pr + 32, vd + 4 * (2048 >> 4), C::kIdescO, 1);
+                    } else {
+                        for (int st = step0; st < step1; ++st)
+                            mma_ts(o, pr + st * 8, vd + st * (2048 >> 4), C::kIdescO, j > 0 || st > step0);
+                    }
+                    if (j + 1 < n_blocks[i]) issue_s(i, k_it);
+                    commit(&s_full[i]);
                 }
-                commit(&s_full[i]);
+                if (!ok) break;
+                commit(&empty[v_it % C::kStages]);
+                if (j + 1 < n_all) commit(&empty[k_it % C::kStages]);
             }
-            if (!ok) break;
-            commit(&empty[v_it % C::kStages]);
-            if (j + 1 < n_all) commit(&empty[k_it % C::kStages]);
+            if (!ok && n_all > 0) *s_abort = 1;
+            commit(done);
+            __all_sync(~0u, tc::wait_bar(done, 0, kDevErrMmaWait));
         }
-        if (!ok && n_all > 0) *s_abort = 1;
-        commit(done);
-        __all_sync(~0u, tc::wait_bar(done, 0, kDevErrMmaWait));
-    }
     } else {
-        // ----------------------------------------------------------------- softmax, one row a thread
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-        const int i = warp >> 2, r = threadIdx.x & 127;
+        // ----------------------------------------------------------------- softmax, two threads a row
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+        const int i = warp >> 3, half = (warp >> 2) & 1, r = threadIdx.x & 127;
         const int my_rows = min(tile_rows, rows - i * tile_rows);
         const int row = first_row + i * tile_rows + r;
         const bool real = r < my_rows;
@@ -327,24 +377,26 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
             row_range(p, s, pos, &row_lo, &row_hi);
             if (MOD && p.slopes) slope = p.slopes[kvh * p.group + row % p.group] * kLog2e;
         }
+        float* mine = reinterpret_cast<float*>(smem + C::kOffRow) + threadIdx.x;          // this thread's place
+        float* other = reinterpret_cast<float*>(smem + C::kOffRow) + (threadIdx.x ^ 128);  // its row's other half
         const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;   // this warp's 32 tensor-memory lanes
-        const uint32_t ts = tmem + lanes + i * kKeys, to = tmem + lanes + C::kTmemO + i * HD;
+        const uint32_t ts = tmem + lanes + i * kKeys, to = tmem + lanes + C::kTmemO + i * HD + half * (HD / 2);
         const float unit = MOD ? 1.0f : p.scale_log2;
         float m = -INFINITY, l = 0.0f;
-        bool ok = true;
         for (int j = 0; j < n_blocks[i]; ++j) {
-            ok = __all_sync(~0u, tc::wait_bar(&s_full[i], j & 1, kDevErrMmaWait) && !*s_abort);
-            if (!ok) break;
+            // after a timeout anywhere no wait is entered, but the group's barriers are all met
+            wait_or_abort(&s_full[i], j & 1, s_abort, kDevErrMmaWait);
+            __syncwarp();
             tc::tc_fence_after();
-            uint32_t sc[4][32];
+            uint32_t sc[2][32];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) tc::tmem_ld32(ts + 32 * q, sc[q]);
+            for (int q = 0; q < 2; ++q) tc::tmem_ld32(ts + half * kHalf + 32 * q, sc[q]);
             tc::tc_wait_ld();
-            const int t0 = seg_lo + j * kKeys;
+            const int t0 = seg_lo + j * kKeys + half * kHalf;
             if constexpr (MOD) {
                 if (p.cap > 0.0f) {
 #pragma unroll
-                    for (int e = 0; e < kKeys; e += 2) {
+                    for (int e = 0; e < kHalf; e += 2) {
                         uint32_t &u0 = sc[e / 32][e % 32], &u1 = sc[e / 32][e % 32 + 1];
                         const float2 t = capped_log2(p, __uint_as_float(u0), __uint_as_float(u1));
                         u0 = __float_as_uint(t.x);
@@ -352,30 +404,36 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
                     }
                 } else {
 #pragma unroll
-                    for (int e = 0; e < kKeys; ++e) sc[e / 32][e % 32] = __float_as_uint(__uint_as_float(sc[e / 32][e % 32]) * p.scale_log2);
+                    for (int e = 0; e < kHalf; ++e) sc[e / 32][e % 32] = __float_as_uint(__uint_as_float(sc[e / 32][e % 32]) * p.scale_log2);
                 }
                 if (p.slopes) {
                     const float dist = static_cast<float>(pos - t0);
 #pragma unroll
-                    for (int e = 0; e < kKeys; ++e)
+                    for (int e = 0; e < kHalf; ++e)
                         sc[e / 32][e % 32] = __float_as_uint(fmaf(-slope, fabsf(dist - static_cast<float>(e)), __uint_as_float(sc[e / 32][e % 32])));
                 }
             }
-            if (__any_sync(~0u, t0 < row_lo || t0 + kKeys > row_hi)) {
+            if (__any_sync(~0u, t0 < row_lo || t0 + kHalf > row_hi)) {
                 const int lo = row_lo - t0, hi = row_hi - t0;
 #pragma unroll
-                for (int e = 0; e < kKeys; ++e)
+                for (int e = 0; e < kHalf; ++e)
                     if (e < lo || e >= hi) sc[e / 32][e % 32] = 0xff800000u;
             }
             float mx[4];
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                mx[q] = fmaxf(__uint_as_float(sc[q][0]), __uint_as_float(sc[q][1]));
+                const uint32_t* u = &sc[q / 2][q % 2 * 16];
+                mx[q] = fmaxf(__uint_as_float(u[0]), __uint_as_float(u[1]));
 #pragma unroll
-                for (int e = 2; e < 32; e += 2) mx[q] = max3(mx[q], __uint_as_float(sc[q][e]), __uint_as_float(sc[q][e + 1]));
+                for (int e = 2; e < 16; e += 2) mx[q] = max3(mx[q], __uint_as_float(u[e]), __uint_as_float(u[e + 1]));
             }
-            const float mn = fmaxf(m, unit * fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
-            if (__any_sync(~0u, mn > m + 8.0f)) {
+            float mn = fmaxf(m, unit * fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+            // Whether any row of the tile needs a new maximum.  The barrier also says that every
+            // score of the tile is in registers, so that probabilities may be written over them.
+            if (group_any(1 + i, mn > m + 8.0f)) {
+                *mine = mn;
+                named_barrier(1 + i, 256);
+                mn = fmaxf(mn, *other);
                 const float f = mn == -INFINITY ? 1.0f : ex2(m - mn);
                 l *= f;
                 m = mn;
@@ -383,12 +441,12 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
                     // the product of the last block is done: its commit came with these scores
 #pragma unroll
                     for (int q = 0; q < HD / 32; ++q) {
-                        uint32_t o[32];
-                        tc::tmem_ld32(to + 32 * q, o);
+                        uint32_t o[32], w[16];   // sixteen columns at a time: the scores hold their registers
+                        tc::tmem_ld16(to + 16 * q, o);
                         tc::tc_wait_ld();
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                        tc::tmem_st32(to + 32 * q, o);
+                        for (int e = 0; e < 16; ++e) w[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                        tc::tmem_st16(to + 16 * q, w);
                     }
                 }
             }
@@ -396,7 +454,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
             const float2 unit2 = make_float2(unit, unit), off2 = make_float2(-off, -off);
             float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
+            for (int q = 0; q < 2; ++q) {
                 uint32_t pk[16];
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
@@ -406,7 +464,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
                     sum = add2(sum, x);
                     pk[e] = pack_bf16(x.x, x.y);
                 }
-                tc::tmem_st16(ts + 16 * q, pk);
+                tc::tmem_st16(ts + half * (kHalf / 2) + 16 * q, pk);
             }
             l += sum.x + sum.y;
             tc::tc_wait_st();
@@ -414,18 +472,23 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
             __syncwarp();
             if (lane == 0) mbar_arrive(&p_full[i]);
         }
-        if (ok && n_blocks[i] > 0) {
-            ok = __all_sync(~0u, tc::wait_bar(&s_full[i], n_blocks[i] & 1, kDevErrMmaWait) && !*s_abort);
+        if (n_blocks[i] > 0) {
+            wait_or_abort(&s_full[i], n_blocks[i] & 1, s_abort, kDevErrMmaWait);
+            __syncwarp();
             tc::tc_fence_after();
         }
-        if (!ok) *s_abort = 1;
-        if (ok && my_rows > 0) {
+        // the row's sum over both halves
+        named_barrier(1 + i, 256);
+        *mine = l;
+        named_barrier(1 + i, 256);
+        l = half ? *other + l : l + *other;   // in one order
+        if (my_rows > 0) {
             const int64_t token = s.q0 + row / p.group, head = kvh * p.group + row % p.group;
             const int D = c.head_dim;
             const int64_t at = split * part.rows + token * p.q_heads + head;
-            if (real && range.splits > 1) part.ml[at] = make_float2(m, l);
+            if (real && half == 0 && range.splits > 1) part.ml[at] = make_float2(m, l);
 #pragma unroll
-            for (int q = 0; q < HD / 32; ++q) {
+            for (int q = 0; q < HD / 64; ++q) {
                 uint32_t o[32];
                 if (n_blocks[i] > 0) {
                     tc::tmem_ld32(to + 32 * q, o);
@@ -436,7 +499,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
                 }
 #pragma unroll
                 for (int e = 0; e < 32; e += 8) {
-                    const int d = 32 * q + e;
+                    const int d = half * (HD / 2) + 32 * q + e;
                     if (!real || d >= D) continue;
                     const float4 x = make_float4(__uint_as_float(o[e]), __uint_as_float(o[e + 1]), __uint_as_float(o[e + 2]), __uint_as_float(o[e + 3]));
                     const float4 y = make_float4(__uint_as_float(o[e + 4]), __uint_as_float(o[e + 5]), __uint_as_float(o[e + 6]), __uint_as_float(o[e + 7]));
@@ -455,7 +518,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
     }
     tc::tc_fence_before();
     __syncthreads();
-    if (warp == 9) {
+    if (warp == kMmaWarp) {
         tc::tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
     }
