@@ -28,6 +28,7 @@
 // Every wait is bounded: on a timeout the kernel records the error, drains its copies and MMAs,
 // frees its tensor memory and returns.
 #include <algorithm>
+#include <type_traits>
 
 #include "attention.cuh"
 
@@ -35,9 +36,10 @@ namespace bybycu {
 namespace attn {
 namespace tcore {
 
-constexpr int kThreads = 640;
+constexpr int kThreads = 576;   // 112 registers a thread
 constexpr int kLoadWarp = 16, kMmaWarp = 17;
 constexpr int kHalf = 64;       // keys of a softmax thread
+constexpr int kFma = 7;         // of 16 exponentials that the FMA units take over (ex2_fma)
 constexpr int kRows = 128;      // query rows of a tile (MMA M)
 constexpr int kKeys = 128;      // keys of a block
 constexpr uint32_t kTmemCols = 512;
@@ -47,14 +49,14 @@ struct Cfg {
     static constexpr int kHalves = HD / 64;                              // 128-byte swizzled boxes a row
     static constexpr uint32_t kQTile = kRows * HD * 2;
     static constexpr uint32_t kBlock = kKeys * HD * 2;                   // one K or V block
-    static constexpr int kStages = HD == 128 ? 4 : 8;
+    static constexpr int kStages = HD == 128 ? 5 : 8;
     static constexpr uint32_t kOffRing = 2 * kQTile;
     static constexpr uint32_t kOffBar = kOffRing + kStages * kBlock;
-    // barriers: q; full, empty [stages]; s_full, p_full [2]; done
-    static constexpr uint32_t kNumBars = 1 + 2 * kStages + 4 + 1;
+    // barriers: q; full, empty [stages]; s_full, p_half, p_full [2]; done
+    static constexpr uint32_t kNumBars = 1 + 2 * kStages + 6 + 1;
     static constexpr uint32_t kOffSlot = kOffBar + kNumBars * 8;
-    static constexpr uint32_t kOffRow = kOffSlot + 8;                    // a float per thread of the softmax groups
-    static constexpr uint32_t kSmem = kOffRow + 512 * 4 + 1024;          // + alignment slack
+    static constexpr uint32_t kOffRow = kOffSlot + 8;                    // a float per query row
+    static constexpr uint32_t kSmem = kOffRow + 2 * kRows * 4 + 1024;    // + alignment slack
     static_assert(kSmem <= 227 * 1024 && kSmem > 114 * 1024, "one CTA per SM");
     // instruction descriptors of kind::f16: D fp32, A and B bf16, M = 128
     static constexpr uint32_t kBase = (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(kRows >> 4) << 24);
@@ -95,15 +97,19 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
                  "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
                  ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
-// The same from tensor memory: A 8 columns (16 keys) further each, B 2048 bytes.
+// Probabilities lie over the scores they came from, each half of 64 keys over its own columns:
+// 16-key step st at column p_column(st).
+__device__ __forceinline__ uint32_t p_column(int st) { return (st >> 2) * kHalf + (st & 3) * 8; }
+// The same from tensor memory: the 16-key steps 0, 1, 4 and 5 from `a` and `b` (2048 bytes of V a
+// step), the keys that both halves of a row's threads write first.
 __device__ __forceinline__ void mma_ts4(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile("{\n\t.reg .pred e, p, q;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %2, 0;\n\tsetp.ne.b32 q, %1, 0;\n\t"
                  "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%3], %7, %1, p;\n\t"
                  "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%4], %8, %1, q;\n\t"
                  "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%5], %9, %1, q;\n\t"
                  "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%6], %10, %1, q;\n\t}"
-                 ::"r"(d), "r"(idesc), "r"(accumulate), "r"(a), "r"(a + 8), "r"(a + 16), "r"(a + 24), "l"(b), "l"(b + 128), "l"(b + 256),
-                 "l"(b + 384)
+                 ::"r"(d), "r"(idesc), "r"(accumulate), "r"(a), "r"(a + 8), "r"(a + kHalf), "r"(a + kHalf + 8), "l"(b), "l"(b + 128), "l"(b + 512),
+                 "l"(b + 640)
                  : "memory");
 }
 __device__ __forceinline__ void commit(uint64_t* bar) {
@@ -131,17 +137,23 @@ __device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, vo
     }
 }
 
-// Whether any of the 256 threads of a softmax group says so; their barrier.
-__device__ __forceinline__ bool group_any(uint32_t id, bool mine) {
+__device__ __forceinline__ float max_nan(float a, float b) {   // NaN where either is
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+
+// Whether any thread of a pair of warps says so; their barrier.
+__device__ __forceinline__ bool pair_any(uint32_t id, bool mine) {
     uint32_t any;
-    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, %2, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, %2, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
                  : "=r"(any) : "r"(static_cast<uint32_t>(mine)), "r"(id) : "memory");
     return any != 0;
 }
 
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
 // Two fp32 operations in one instruction.
@@ -159,18 +171,43 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     return d;
 }
 
+// 2^x of two numbers below 128 on the FMA units: x = n + f with n the nearest whole number (the
+// low bits of x + 1.5 * 2^23), 2^f by the cubic of least relative error on [-1/2, 1/2] (7.5e-5, by
+// Remez exchange; a bf16 probability is rounded by up to 3.9e-3 after it), n added to the exponent.
+// Below 2^-125 it stays there: masked scores, whose 2^x has to be 0, do not come here.
+__device__ __forceinline__ float2 ex2_fma(float2 x) {
+    const float magic = 12582912.0f;
+    x.x = fmaxf(x.x, -125.0f);
+    x.y = fmaxf(x.y, -125.0f);
+    const float2 t = add2(x, make_float2(magic, magic));
+    const float2 n = add2(t, make_float2(-magic, -magic));
+    const float2 f = fma2(n, make_float2(-1.0f, -1.0f), x);
+    float2 y = fma2(f, make_float2(0.0551716685f, 0.0551716685f), make_float2(0.242611125f, 0.242611125f));
+    y = fma2(y, f, make_float2(0.693260968f, 0.693260968f));
+    y = fma2(y, f, make_float2(0.999928057f, 0.999928057f));
+    return make_float2(__uint_as_float(__float_as_uint(y.x) + (__float_as_uint(t.x) << 23)),
+                       __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(t.y) << 23)));
+}
+
 template <int HD, bool MOD>
 __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_constant__ Maps maps, const kvc::Cache c,
-                                                                   const Params p, const Partials part, int split_keys,
-                                                                   int tile_rows, int box_slots) {
+                                                                   const Params p, const Partials part, int split_keys, int splits,
+                                                                   int tiles, int band, int tile_rows, int box_slots) {
     using C = Cfg<HD>;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     pdl_launch_dependents();
     pdl_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int kvh = blockIdx.x % c.kv_heads, split = blockIdx.x / c.kv_heads, b = blockIdx.y;
-    // late tiles see the most keys: first
-    const int first_row = static_cast<int>(gridDim.z - 1 - blockIdx.z) * 2 * tile_rows;
+    // Order of the grid: bands of (sequence, kv head, split) whose keys and values fit into L2
+    // together; within a band the late tiles, which see the most keys, come first.
+    const int64_t units = static_cast<int64_t>(c.n_seqs) * c.kv_heads * splits;
+    const int64_t first_unit = blockIdx.x / (static_cast<int64_t>(band) * tiles) * band;
+    const int in_band = static_cast<int>(units - first_unit < band ? units - first_unit : band);
+    const int at = static_cast<int>(blockIdx.x - first_unit * tiles);
+    const int64_t unit_id = first_unit + at % in_band;
+    const int split = static_cast<int>(unit_id % splits), kvh = static_cast<int>(unit_id / splits % c.kv_heads);
+    const int b = static_cast<int>(unit_id / splits / c.kv_heads);
+    const int first_row = (tiles - 1 - at / in_band) * 2 * tile_rows;
     const Seq s = load_seq(c, p, b);
     const int rows = min(2 * tile_rows, s.rows * p.group - first_row);
     if (rows <= 0) return;
@@ -197,7 +234,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
     uint64_t* full = q_full + 1;
     uint64_t* empty = full + C::kStages;
     uint64_t* s_full = empty + C::kStages;   // [2] scores (after the last block: the output) ready
-    uint64_t* p_full = s_full + 2;           // [2] probabilities written, output rescaled
+    uint64_t* p_half = s_full + 2;           // [2] output rescaled, keys 0-31 and 64-95 of the probabilities written
+    uint64_t* p_full = p_half + 2;           // [2] the others written
     uint64_t* done = p_full + 2;
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + C::kOffSlot);
     volatile int* s_abort = reinterpret_cast<volatile int*>(smem + C::kOffSlot + 4);
@@ -209,6 +247,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&s_full[i], 1);
+            mbar_init(&p_half[i], 8);
             mbar_init(&p_full[i], 8);
         }
         mbar_init(done, 1);
@@ -225,10 +264,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
     tc::tc_fence_after();
     const uint32_t tmem = *tmem_slot;
 
-    // The softmax groups take registers from the other four warps (512 * 104 + 128 * 64 = 640 * 96,
-    // what the launch holds).
     if (warp >= kLoadWarp) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
         if (warp == kLoadWarp) {
             // ----------------------------------------------------------------- loads
             if (n_all > 0) {
@@ -341,16 +377,20 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     if (j >= n_blocks[i]) continue;
+                    const uint32_t o = tmem + C::kTmemO + i * HD, pr = tmem + i * kKeys;
+                    const bool whole = step0 == 0 && step1 == kKeys / 16;
+                    ok = __all_sync(~0u, wait_or_abort(&p_half[i], j & 1, s_abort, kDevErrMmaWait));
+                    if (!ok) break;
+                    tc::tc_fence_after();
+                    if (whole) mma_ts4(o, pr, vd, C::kIdescO, j > 0);
                     ok = __all_sync(~0u, wait_or_abort(&p_full[i], j & 1, s_abort, kDevErrMmaWait));
                     if (!ok) break;
                     tc::tc_fence_after();
-                    const uint32_t o = tmem + C::kTmemO + i * HD, pr = tmem + i * kKeys;
-                    if (step0 == 0 && step1 == kKeys / 16) {
-                        mma_ts4(o, pr, vd, C::kIdescO, j > 0);
-                        mma_ts4(o, pr + 32, vd + 4 * (2048 >> 4), C::kIdescO, 1);
+                    if (whole) {
+                        mma_ts4(o, pr + 16, vd + 2 * (2048 >> 4), C::kIdescO, 1);
                     } else {
                         for (int st = step0; st < step1; ++st)
-                            mma_ts(o, pr + st * 8, vd + st * (2048 >> 4), C::kIdescO, j > 0 || st > step0);
+                            mma_ts(o, pr + p_column(st), vd + st * (2048 >> 4), C::kIdescO, j > 0 || st > step0);
                     }
                     if (j + 1 < n_blocks[i]) issue_s(i, k_it);
                     commit(&s_full[i]);
@@ -365,7 +405,6 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
         }
     } else {
         // ----------------------------------------------------------------- softmax, two threads a row
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
         const int i = warp >> 3, half = (warp >> 2) & 1, r = threadIdx.x & 127;
         const int my_rows = min(tile_rows, rows - i * tile_rows);
         const int row = first_row + i * tile_rows + r;
@@ -377,10 +416,17 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
             row_range(p, s, pos, &row_lo, &row_hi);
             if (MOD && p.slopes) slope = p.slopes[kvh * p.group + row % p.group] * kLog2e;
         }
-        float* mine = reinterpret_cast<float*>(smem + C::kOffRow) + threadIdx.x;          // this thread's place
-        float* other = reinterpret_cast<float*>(smem + C::kOffRow) + (threadIdx.x ^ 128);  // its row's other half
+        // f(this thread's value, its row's other value), the same in both: by the second half's thread
+        float* place = reinterpret_cast<float*>(smem + C::kOffRow) + i * kRows + r;
+        auto join = [&](float mine, auto f) {
+            if (half == 0) *place = mine;
+            named_barrier(1 + i * 4 + (warp & 3), 64);
+            if (half == 1) *place = f(*place, mine);
+            named_barrier(1 + i * 4 + (warp & 3), 64);
+            return *place;
+        };
         const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;   // this warp's 32 tensor-memory lanes
-        const uint32_t ts = tmem + lanes + i * kKeys, to = tmem + lanes + C::kTmemO + i * HD + half * (HD / 2);
+        const uint32_t ts = tmem + lanes + i * kKeys + half * kHalf, to = tmem + lanes + C::kTmemO + i * HD + half * (HD / 2);
         const float unit = MOD ? 1.0f : p.scale_log2;
         float m = -INFINITY, l = 0.0f;
         for (int j = 0; j < n_blocks[i]; ++j) {
@@ -388,52 +434,58 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
             wait_or_abort(&s_full[i], j & 1, s_abort, kDevErrMmaWait);
             __syncwarp();
             tc::tc_fence_after();
-            uint32_t sc[2][32];
-#pragma unroll
-            for (int q = 0; q < 2; ++q) tc::tmem_ld32(ts + half * kHalf + 32 * q, sc[q]);
-            tc::tc_wait_ld();
             const int t0 = seg_lo + j * kKeys + half * kHalf;
-            if constexpr (MOD) {
-                if (p.cap > 0.0f) {
+            // 32 of this thread's scores, in the units of the sum to come, -inf where the row may not look
+            auto load = [&](int q, uint32_t (&sc)[32]) {
+                tc::tmem_ld32(ts + 32 * q, sc);
+                tc::tc_wait_ld();
+                if constexpr (MOD) {
+                    if (p.cap > 0.0f) {
 #pragma unroll
-                    for (int e = 0; e < kHalf; e += 2) {
-                        uint32_t &u0 = sc[e / 32][e % 32], &u1 = sc[e / 32][e % 32 + 1];
-                        const float2 t = capped_log2(p, __uint_as_float(u0), __uint_as_float(u1));
-                        u0 = __float_as_uint(t.x);
-                        u1 = __float_as_uint(t.y);
+                        for (int e = 0; e < 32; e += 2) {
+                            const float2 t = capped_log2(p, __uint_as_float(sc[e]), __uint_as_float(sc[e + 1]));
+                            sc[e] = __float_as_uint(t.x);
+                            sc[e + 1] = __float_as_uint(t.y);
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) sc[e] = __float_as_uint(__uint_as_float(sc[e]) * p.scale_log2);
                     }
-                } else {
+                    if (p.slopes) {
+                        const float dist = static_cast<float>(pos - t0 - 32 * q);
 #pragma unroll
-                    for (int e = 0; e < kHalf; ++e) sc[e / 32][e % 32] = __float_as_uint(__uint_as_float(sc[e / 32][e % 32]) * p.scale_log2);
+                        for (int e = 0; e < 32; ++e)
+                            sc[e] = __float_as_uint(fmaf(-slope, fabsf(dist - static_cast<float>(e)), __uint_as_float(sc[e])));
+                    }
                 }
-                if (p.slopes) {
-                    const float dist = static_cast<float>(pos - t0);
+                const int lo = row_lo - t0 - 32 * q, hi = row_hi - t0 - 32 * q;
+                const bool masked = __any_sync(~0u, lo > 0 || hi < 32);
+                if (masked) {
 #pragma unroll
-                    for (int e = 0; e < kHalf; ++e)
-                        sc[e / 32][e % 32] = __float_as_uint(fmaf(-slope, fabsf(dist - static_cast<float>(e)), __uint_as_float(sc[e / 32][e % 32])));
+                    for (int e = 0; e < 32; ++e)
+                        if (e < lo || e >= hi) sc[e] = 0xff800000u;
                 }
-            }
-            if (__any_sync(~0u, t0 < row_lo || t0 + kHalf > row_hi)) {
-                const int lo = row_lo - t0, hi = row_hi - t0;
+                return masked;
+            };
+            auto top = [&](const uint32_t (&sc)[32]) {
+                float mx[4];
 #pragma unroll
-                for (int e = 0; e < kHalf; ++e)
-                    if (e < lo || e >= hi) sc[e / 32][e % 32] = 0xff800000u;
-            }
-            float mx[4];
+                for (int q = 0; q < 4; ++q) {
+                    mx[q] = max_nan(__uint_as_float(sc[q]), __uint_as_float(sc[q + 4]));
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const uint32_t* u = &sc[q / 2][q % 2 * 16];
-                mx[q] = fmaxf(__uint_as_float(u[0]), __uint_as_float(u[1]));
-#pragma unroll
-                for (int e = 2; e < 16; e += 2) mx[q] = max3(mx[q], __uint_as_float(u[e]), __uint_as_float(u[e + 1]));
-            }
-            float mn = fmaxf(m, unit * fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
-            // Whether any row of the tile needs a new maximum.  The barrier also says that every
-            // score of the tile is in registers, so that probabilities may be written over them.
-            if (group_any(1 + i, mn > m + 8.0f)) {
-                *mine = mn;
-                named_barrier(1 + i, 256);
-                mn = fmaxf(mn, *other);
+                    for (int e = q + 8; e < 32; e += 8) mx[q] = e + 4 < 32 ? max3(mx[q], __uint_as_float(sc[e]), __uint_as_float(sc[e + 4])) : mx[q];
+                }
+                return max_nan(max3(mx[0], mx[1], mx[2]), mx[3]);
+            };
+            // The first 32 scores stay in registers, the second come again after the maximum is
+            // known (registers left free let the exponentials overlap), unless they took work.
+            uint32_t first[32], second[32];
+            const bool masked0 = load(0, first);
+            bool masked1 = load(1, second);
+            float mn = max_nan(m, unit * max_nan(top(first), top(second)));   // a NaN score makes the row NaN
+            // Whether a row of this pair of warps (the two halves of 32 rows) needs a new maximum
+            if (pair_any(1 + i * 4 + (warp & 3), !(mn <= m + 8.0f) && mn != -INFINITY)) {
+                mn = join(mn, [](float a, float b) { return max_nan(a, b); });
                 const float f = mn == -INFINITY ? 1.0f : ex2(m - mn);
                 l *= f;
                 m = mn;
@@ -453,35 +505,41 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
             const float off = m == -INFINITY ? 0.0f : m;
             const float2 unit2 = make_float2(unit, unit), off2 = make_float2(-off, -off);
             float2 sum = make_float2(0.0f, 0.0f);
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
+            // 32 probabilities over the first 16 (q = 0) or the next 16 columns of this half's scores
+            auto probabilities = [&](const uint32_t (&sc)[32], int q, auto split) {
                 uint32_t pk[16];
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    float2 x = fma2(make_float2(__uint_as_float(sc[q][2 * e]), __uint_as_float(sc[q][2 * e + 1])), unit2, off2);
-                    x.x = ex2(x.x);
-                    x.y = ex2(x.y);
+                    float2 x = fma2(make_float2(__uint_as_float(sc[2 * e]), __uint_as_float(sc[2 * e + 1])), unit2, off2);
+                    if (decltype(split)::value && e * kFma / 16 != (e + 1) * kFma / 16) {
+                        x = ex2_fma(x);
+                    } else {
+                        x.x = ex2(x.x);
+                        x.y = ex2(x.y);
+                    }
                     sum = add2(sum, x);
                     pk[e] = pack_bf16(x.x, x.y);
                 }
-                tc::tmem_st16(ts + half * (kHalf / 2) + 16 * q, pk);
-            }
+                tc::tmem_st16(ts + 16 * q, pk);
+                tc::tc_wait_st();
+                tc::tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(q ? &p_full[i] : &p_half[i]);   // the tensor core starts on the first 32
+            };
+            if (masked0) probabilities(first, 0, std::false_type{});
+            else probabilities(first, 0, std::true_type{});
+            if constexpr (!MOD) masked1 = load(1, second);
+            if (masked1) probabilities(second, 1, std::false_type{});
+            else probabilities(second, 1, std::true_type{});
             l += sum.x + sum.y;
-            tc::tc_wait_st();
-            tc::tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[i]);
         }
         if (n_blocks[i] > 0) {
             wait_or_abort(&s_full[i], n_blocks[i] & 1, s_abort, kDevErrMmaWait);
             __syncwarp();
             tc::tc_fence_after();
         }
-        // the row's sum over both halves
-        named_barrier(1 + i, 256);
-        *mine = l;
-        named_barrier(1 + i, 256);
-        l = half ? *other + l : l + *other;   // in one order
+        named_barrier(1 + i * 4 + (warp & 3), 64);   // every place has been read
+        l = join(l, [](float a, float b) { return a + b; });
         if (my_rows > 0) {
             const int64_t token = s.q0 + row / p.group, head = kvh * p.group + row % p.group;
             const int D = c.head_dim;
@@ -582,16 +640,19 @@ static int launch(const kvc::Cache& c, const Params& p, const DeviceInfo& info, 
     const int64_t split_keys64 = std::max<int64_t>(ceil_div(ceil_div(span, splits), kKeys) * kKeys, 4 * kKeys);
     splits = splits == 1 ? 1 : ceil_div(span, split_keys64);
     const int split_keys = splits == 1 ? INT32_MAX / 2 / kKeys * kKeys : static_cast<int>(split_keys64);
-    if (tiles > 65535 || c.n_seqs > 65535 || splits * c.kv_heads > INT32_MAX)
+    if (units * splits > INT32_MAX)
         return set_error(BYBYCU_ERR_SHAPE, "paged_attention: %d sequences, %d kv heads, %d new tokens", c.n_seqs, c.kv_heads, p.max_q);
     Partials part{};
     SplitScratchMem scratch;
     if (splits > 1)
         if (int rc = scratch.take(info.device, static_cast<int64_t>(c.n_tokens) * p.q_heads, static_cast<int>(splits), c.head_dim, stream, &part)) return rc;
     cudaLaunchAttribute attr[1];
-    const cudaLaunchConfig_t cfg = pdl_config(dim3(static_cast<unsigned>(splits * c.kv_heads), static_cast<unsigned>(c.n_seqs),
-                                                   static_cast<unsigned>(tiles)), kThreads, C::kSmem, stream, attr);
-    BYBYCU_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, maps, c, p, part, split_keys, tile_rows, box_slots));
+    // K and V of a band: about half of the 126 MB L2
+    const int64_t unit_bytes = std::min<int64_t>(span, split_keys) * c.head_dim * 4;
+    const int band = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((64 << 20) / unit_bytes, 1 << 20)));
+    const cudaLaunchConfig_t cfg = pdl_config(dim3(static_cast<unsigned>(units * splits)), kThreads, C::kSmem, stream, attr);
+    BYBYCU_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, maps, c, p, part, split_keys, static_cast<int>(splits), static_cast<int>(tiles), band,
+                                       tile_rows, box_slots));
     return splits > 1 ? launch_join(c, p, part, split_keys, 2 * tile_rows, kKeys, false, stream) : BYBYCU_OK;
 }
 
