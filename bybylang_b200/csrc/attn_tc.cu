@@ -39,7 +39,8 @@ namespace tcore {
 constexpr int kThreads = 576;   // 112 registers a thread
 constexpr int kLoadWarp = 16, kMmaWarp = 17;
 constexpr int kHalf = 64;       // keys of a softmax thread
-constexpr int kFma = 7;         // of 16 exponentials that the FMA units take over (ex2_fma)
+constexpr int kFma = 3;         // of 16 exponentials that the FMA units take over: 0, 2, 4, 5, 7 of 16
+                                // measured 267, 265, 266, 267, 272 us (2 x 4096 tokens, 32/8 heads of 128)
 constexpr int kRows = 128;      // query rows of a tile (MMA M)
 constexpr int kKeys = 128;      // keys of a block
 constexpr uint32_t kTmemCols = 512;
@@ -100,16 +101,15 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
 // Probabilities lie over the scores they came from, each half of 64 keys over its own columns:
 // 16-key step st at column p_column(st).
 __device__ __forceinline__ uint32_t p_column(int st) { return (st >> 2) * kHalf + (st & 3) * 8; }
-// The same from tensor memory: the 16-key steps 0, 1, 4 and 5 from `a` and `b` (2048 bytes of V a
-// step), the keys that both halves of a row's threads write first.
+// The same from tensor memory: four 16-key steps from `a` and `b` (2048 bytes of V a step).
 __device__ __forceinline__ void mma_ts4(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile("{\n\t.reg .pred e, p, q;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %2, 0;\n\tsetp.ne.b32 q, %1, 0;\n\t"
                  "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%3], %7, %1, p;\n\t"
                  "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%4], %8, %1, q;\n\t"
                  "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%5], %9, %1, q;\n\t"
                  "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%6], %10, %1, q;\n\t}"
-                 ::"r"(d), "r"(idesc), "r"(accumulate), "r"(a), "r"(a + 8), "r"(a + kHalf), "r"(a + kHalf + 8), "l"(b), "l"(b + 128), "l"(b + 512),
-                 "l"(b + 640)
+                 ::"r"(d), "r"(idesc), "r"(accumulate), "r"(a), "r"(a + 8), "r"(a + 16), "r"(a + 24), "l"(b), "l"(b + 128), "l"(b + 256),
+                 "l"(b + 384)
                  : "memory");
 }
 __device__ __forceinline__ void commit(uint64_t* bar) {
@@ -234,8 +234,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
     uint64_t* full = q_full + 1;
     uint64_t* empty = full + C::kStages;
     uint64_t* s_full = empty + C::kStages;   // [2] scores (after the last block: the output) ready
-    uint64_t* p_half = s_full + 2;           // [2] output rescaled, keys 0-31 and 64-95 of the probabilities written
-    uint64_t* p_full = p_half + 2;           // [2] the others written
+    uint64_t* p_half = s_full + 2;           // [2] output rescaled, probabilities of keys 0-63 written
+    uint64_t* p_full = p_half + 2;           // [2] of keys 64-127
     uint64_t* done = p_full + 2;
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + C::kOffSlot);
     volatile int* s_abort = reinterpret_cast<volatile int*>(smem + C::kOffSlot + 4);
@@ -247,8 +247,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&s_full[i], 1);
-            mbar_init(&p_half[i], 8);
-            mbar_init(&p_full[i], 8);
+            mbar_init(&p_half[i], 4);
+            mbar_init(&p_full[i], 4);
         }
         mbar_init(done, 1);
         *s_abort = 0;
@@ -387,7 +387,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
                     if (!ok) break;
                     tc::tc_fence_after();
                     if (whole) {
-                        mma_ts4(o, pr + 16, vd + 2 * (2048 >> 4), C::kIdescO, 1);
+                        mma_ts4(o, pr + kHalf, vd + 4 * (2048 >> 4), C::kIdescO, 1);
                     } else {
                         for (int st = step0; st < step1; ++st)
                             mma_ts(o, pr + p_column(st), vd + st * (2048 >> 4), C::kIdescO, j > 0 || st > step0);
@@ -426,7 +426,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
             return *place;
         };
         const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;   // this warp's 32 tensor-memory lanes
-        const uint32_t ts = tmem + lanes + i * kKeys + half * kHalf, to = tmem + lanes + C::kTmemO + i * HD + half * (HD / 2);
+        const uint32_t ts = tmem + lanes + i * kKeys + half * kHalf, to = tmem + lanes + C::kTmemO + i * HD;
         const float unit = MOD ? 1.0f : p.scale_log2;
         float m = -INFINITY, l = 0.0f;
         for (int j = 0; j < n_blocks[i]; ++j) {
@@ -489,10 +489,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
                 const float f = mn == -INFINITY ? 1.0f : ex2(m - mn);
                 l *= f;
                 m = mn;
-                if (j > 0) {
+                if (j > 0 && half == 0) {
                     // the product of the last block is done: its commit came with these scores
 #pragma unroll
-                    for (int q = 0; q < HD / 32; ++q) {
+                    for (int q = 0; q < HD / 16; ++q) {
                         uint32_t o[32], w[16];   // sixteen columns at a time: the scores hold their registers
                         tc::tmem_ld16(to + 16 * q, o);
                         tc::tc_wait_ld();
@@ -521,16 +521,18 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
                     pk[e] = pack_bf16(x.x, x.y);
                 }
                 tc::tmem_st16(ts + 16 * q, pk);
-                tc::tc_wait_st();
-                tc::tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(q ? &p_full[i] : &p_half[i]);   // the tensor core starts on the first 32
             };
             if (masked0) probabilities(first, 0, std::false_type{});
             else probabilities(first, 0, std::true_type{});
             if constexpr (!MOD) masked1 = load(1, second);
             if (masked1) probabilities(second, 1, std::false_type{});
             else probabilities(second, 1, std::true_type{});
+            tc::tc_wait_st();
+            tc::tc_fence_before();
+            __syncwarp();
+            // of two warps on a scheduler the lower one runs ahead: keys 0-63 are done first, and
+            // the tensor core starts on them
+            if (lane == 0) mbar_arrive(half ? &p_full[i] : &p_half[i]);
             l += sum.x + sum.y;
         }
         if (n_blocks[i] > 0) {
@@ -549,7 +551,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
             for (int q = 0; q < HD / 64; ++q) {
                 uint32_t o[32];
                 if (n_blocks[i] > 0) {
-                    tc::tmem_ld32(to + 32 * q, o);
+                    tc::tmem_ld32(to + half * (HD / 2) + 32 * q, o);
                     tc::tc_wait_ld();
                 } else {
 #pragma unroll
