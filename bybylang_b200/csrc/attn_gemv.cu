@@ -422,15 +422,17 @@ if constexpr (F32) {
     }
 }
 
-// Joins the splits: one warp a row (token, head), splits in order.
+// Joins the splits: a block a row (token, head), each warp a quarter of the splits, then the four
+// in order.
 template <bool F32>
 __global__ void __launch_bounds__(128) attention_join_kernel(const kvc::Cache c, const Params p, const Partials part,
                                                              int split_keys, int tile_rows, int align) {
+    __shared__ float s_sum[4];
+    __shared__ float4 s_acc[3][kvc::kMaxHeadDim / 4];
     pdl_launch_dependents();
     pdl_wait();
-    const int lane = threadIdx.x & 31;
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-    if (row >= part.rows) return;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t row = blockIdx.x;
     const int t = static_cast<int>(row / p.q_heads), h = static_cast<int>(row % p.q_heads), D = c.head_dim;
     int b = 0;
     for (int i = 0; i < c.n_seqs; i += 32) b += __popc(__ballot_sync(~0u, i + lane < c.n_seqs && c.q_start[i + lane + 1] <= t));
@@ -446,21 +448,35 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const kvc::Cache c,
 #pragma unroll
     for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, o));
     const float base = mx == -INFINITY ? 0.0f : mx;
-    for (int d = lane * 4; d < D; d += 128) {
+    const int per = (range.splits + 3) / 4, k0 = warp * per, k1 = min(range.splits, k0 + per);
+    for (int d0 = 0; d0 < D; d0 += 128) {
+        const int d = d0 + lane * 4;
         float sum = 0.0f;
         float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (d < D) {
 #pragma unroll 4
-        for (int k = 0; k < range.splits; ++k) {
-            const float2 ml = part.ml[k * part.rows + row];
-            const float4 v = *reinterpret_cast<const float4*>(part.o + (k * part.rows + row) * D + d);
-            const float f = exp2f(ml.x - base);
-            sum = fmaf(f, ml.y, sum);
-            acc.x = fmaf(f, v.x, acc.x);
-            acc.y = fmaf(f, v.y, acc.y);
-            acc.z = fmaf(f, v.z, acc.z);
-            acc.w = fmaf(f, v.w, acc.w);
+            for (int k = k0; k < k1; ++k) {
+                const float2 ml = part.ml[k * part.rows + row];
+                const float4 v = *reinterpret_cast<const float4*>(part.o + (k * part.rows + row) * D + d);
+                const float f = exp2f(ml.x - base);
+                sum = fmaf(f, ml.y, sum);
+                acc.x = fmaf(f, v.x, acc.x);
+                acc.y = fmaf(f, v.y, acc.y);
+                acc.z = fmaf(f, v.z, acc.z);
+                acc.w = fmaf(f, v.w, acc.w);
+            }
+            if (warp) s_acc[warp - 1][d / 4] = acc;
         }
-        store_row4<F32>(p, t, h, d, acc, sum);
+        if (lane == 0) s_sum[warp] = sum;
+        __syncthreads();
+        if (warp == 0 && d < D) {
+            for (int w = 0; w < 3; ++w) {
+                const float4 v = s_acc[w][d / 4];
+                acc = make_float4(acc.x + v.x, acc.y + v.y, acc.z + v.z, acc.w + v.w);
+            }
+            store_row4<F32>(p, t, h, d, acc, s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3]);
+        }
+        __syncthreads();
     }
 }
 
@@ -481,7 +497,7 @@ static cudaLaunchConfig_t pdl_config(dim3 grid, int threads, size_t smem, cudaSt
 static int launch_join(const kvc::Cache& c, const Params& p, const Partials& part, int split_keys, int tile_rows,
                        int align, bool f32, cudaStream_t stream) {
     cudaLaunchAttribute attr[1];
-    const cudaLaunchConfig_t cfg = pdl_config(dim3(static_cast<unsigned>(ceil_div(part.rows, 4))), 128, 0, stream, attr);
+    const cudaLaunchConfig_t cfg = pdl_config(dim3(static_cast<unsigned>(part.rows)), 128, 0, stream, attr);
     BYBYCU_CUDA_TRY(cudaLaunchKernelEx(&cfg, f32 ? attention_join_kernel<true> : attention_join_kernel<false>, c, p, part,
                                        split_keys, tile_rows, align));
     return BYBYCU_OK;

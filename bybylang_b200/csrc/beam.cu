@@ -2,9 +2,10 @@
 //
 // score(b, t) = scores[b] + (x[b][t] - lse[b]), lse[b] = m + log(sum_t exp(x[b][t] - m)): every
 // logit is needed once for the sum, and the order of a beam's continuations is the order of its
-// logits.  So one pass over the logits does both: a block reads one slice of one row into
-// registers, reduces its maximum and sum, and keeps the slice's `keep` largest logits; a second,
-// small kernel joins the slices of each row and then the beams of each group.
+// logits.  So one pass over the logits does both: a block walks one slice of one row, each thread
+// with a running maximum and sum, and collects the logits that can still be among the slice's
+// `keep` largest; a second, small kernel joins the slices of each row and then the beams of each
+// group.
 //
 // Order is kept in whole numbers: a candidate is the 64-bit key (ordered bits of the logit, then
 // the complement of the token), so no two keys are equal, equal logits go to the lower token and
@@ -22,13 +23,18 @@ namespace beam {
 constexpr int kThreads = 256;
 constexpr int kMaxKeep = 64;
 constexpr int kMaxSlices = 128;
-constexpr int kCand = 512;      // candidates of a slice that are ranked against each other
+constexpr int kItems = 8;                     // logits of a thread in one chunk
+constexpr int kChunk = kThreads * kItems;     // 2048
+constexpr int kSoft = 256;                    // candidates above which they are cut down to the best `keep`
+constexpr int kCand = kSoft + kChunk;         // so that a whole chunk always finds room
+constexpr int kRanked = 512;                  // candidates that are ranked against each other; more are bisected first
+static_assert(kSoft >= 2 * kMaxKeep, "a cut has to make room");
 
 struct Params {
     const void* x;
     int64_t row_stride;
     const float* scores;
-    int groups, beams, vocab, keep, slices;
+    int groups, beams, vocab, keep, slices, slice_len;   // slice_len: a multiple of kChunk
     float2* part;        // [rows][slices] maximum and sum of a slice
     uint64_t* keys;      // [rows][slices][keep] the slice's best, best first; 0 = none
     float* out_scores;
@@ -44,142 +50,196 @@ __device__ __forceinline__ float from_ordered(uint32_t u) {
     return __uint_as_float(u ^ ((u >> 31) ? 0x80000000u : 0xffffffffu));
 }
 
-// One slice of kThreads * ITEMS logits of one row, in registers.  Which of them can be among the
-// slice's `keep` largest: every warp whose 32 threads all have tokens takes the r-th largest of
-// its threads' own maxima, r = ceil(keep / warps); at least keep keys are not below the smallest
-// of these, so it bounds the result from below, and for logits in no particular order some 2 *
-// keep elements reach it.  Where more than kCand do (a warp whose tokens are all masked, a slice
-// too short for a bound), a bisection over the keys finds the exact bound instead.
-template <typename T, int ITEMS, bool VEC>
-__global__ void __launch_bounds__(kThreads) beam_scan_kernel(const Params p) {
+// Cuts the n candidates of s_cand down to the best `keep`, sorted; the new count, the same for
+// every thread.  Ranks by counting; more than kRanked are first bisected down to exactly `keep`,
+// one key bit at a time.
+__device__ __forceinline__ int cut(uint64_t* s_cand, int* s_count, int* s_part, int n, int keep) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    constexpr int kWarps = kThreads / 32, kMine = (kCand + kThreads - 1) / kThreads;
+    if (n > kRanked) {
+        uint64_t bound = 0;
+        for (int bit = 63; bit >= 0; --bit) {
+            const uint64_t tried = bound | (1ull << bit);
+            int c = 0;
+            for (int i = tid; i < n; i += kThreads) c += s_cand[i] >= tried;
+            c = __reduce_add_sync(~0u, c);
+            if (lane == 0) s_part[warp] = c;
+            __syncthreads();
+            c = 0;
+            for (int w = 0; w < kWarps; ++w) c += s_part[w];
+            __syncthreads();
+            if (c >= keep) bound = tried;
+        }
+        uint64_t mine[kMine];
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) mine[i] = i * kThreads + tid < n ? s_cand[i * kThreads + tid] : 0;
+        if (tid == 0) *s_count = 0;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kMine; ++i)
+            if (mine[i] >= bound && mine[i] != 0) s_cand[atomicAdd(s_count, 1)] = mine[i];
+        __syncthreads();
+        n = *s_count;
+    }
+    uint64_t k[kRanked / kThreads];
+    int rank[kRanked / kThreads] = {};
+#pragma unroll
+    for (int i = 0; i < kRanked / kThreads; ++i) k[i] = i * kThreads + tid < n ? s_cand[i * kThreads + tid] : 0;
+    for (int j = 0; j < n; ++j) {
+        const uint64_t o = s_cand[j];
+#pragma unroll
+        for (int i = 0; i < kRanked / kThreads; ++i) rank[i] += o > k[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kRanked / kThreads; ++i)
+        if (i * kThreads + tid < n && rank[i] < keep) s_cand[rank[i]] = k[i];
+    n = min(n, keep);
+    if (tid == 0) *s_count = n;
+    __syncthreads();
+    return n;
+}
+
+// One slice of one row, chunk by chunk.  A logit is a candidate when it is not below the bound,
+// the keep-th best so far; the first chunk has a bound to start from: every warp takes the r-th
+// largest of its threads' own maxima, r = ceil(keep / warps), and at least keep keys are not below
+// the smallest of these.  For logits in no particular order some 2 * keep elements of the first
+// chunk and keep / c of the c-th become candidates.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kThreads, 4) beam_scan_kernel(const Params p) {
     __shared__ uint64_t s_cand[kCand];
-    __shared__ float s_red[2][kThreads / 32];
     __shared__ uint64_t s_bound[kThreads / 32];
+    __shared__ float s_max[kThreads / 32], s_sum[kThreads / 32];
+    __shared__ int s_part[kThreads / 32];
     __shared__ int s_count;
     pdl_launch_dependents();
     pdl_wait();
-    constexpr int kVec = VEC ? 16 / static_cast<int>(sizeof(T)) : 1;
+    constexpr int kVec = VEC ? 16 / static_cast<int>(sizeof(T)) : 1, kLoads = kItems / kVec;
     constexpr int kWarps = kThreads / 32;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int row = blockIdx.y, slice = blockIdx.x;
-    const int base = slice * (kThreads * ITEMS);
+    const int lo = slice * p.slice_len, hi = min(p.vocab, lo + p.slice_len);
     const T* x = static_cast<const T*>(p.x) + row * p.row_stride;
-    // a thread's tokens ascend with i
-    auto token = [&](int i) { return base + (i / kVec * kThreads + tid) * kVec + i % kVec; };
+    // a thread's tokens of a chunk ascend with i
+    auto token = [&](int c, int i) { return lo + c * kChunk + (i / kVec * kThreads + tid) * kVec + i % kVec; };
     auto key = [&](float v, int t) { return (static_cast<uint64_t>(ordered_bits(v)) << 32) | ~static_cast<uint32_t>(t); };
-    float v[ITEMS];
+    auto fetch = [&](int c, uint4 (&raw)[kLoads]) {   // whole vectors only; the ragged end is read by itself
+        if constexpr (VEC) {
 #pragma unroll
-    for (int i = 0; i < ITEMS; i += kVec) {
-        const int t = token(i);
-        if (VEC && t + kVec <= p.vocab) {
-            const uint4 w = __ldcs(reinterpret_cast<const uint4*>(x + t));
-            const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+            for (int i = 0; i < kLoads; ++i)
+                if (token(c, i * kVec) + kVec <= hi) raw[i] = __ldcs(reinterpret_cast<const uint4*>(x + token(c, i * kVec)));
+        }
+    };
+    auto unpack = [&](int c, const uint4 (&raw)[kLoads], float (&v)[kItems]) {
 #pragma unroll
-            for (int e = 0; e < kVec; ++e) {
-                if constexpr (sizeof(T) == 4) v[i + e] = __uint_as_float(u[e % 4]);
-                else v[i + e] = __uint_as_float(e & 1 ? u[e / 2 % 4] & 0xffff0000u : u[e / 2 % 4] << 16);
+        for (int i = 0; i < kLoads; ++i) {
+            if (VEC && token(c, i * kVec) + kVec <= hi) {
+                const uint32_t u[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+                for (int e = 0; e < kVec; ++e) {
+                    if constexpr (sizeof(T) == 4) v[i * kVec + e] = __uint_as_float(u[e % 4]);
+                    else v[i * kVec + e] = __uint_as_float(e & 1 ? u[e / 2 % 4] & 0xffff0000u : u[e / 2 % 4] << 16);
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < kVec; ++e) {
+                    const int t = token(c, i * kVec + e);
+                    v[i * kVec + e] = t < hi ? static_cast<float>(x[t]) : -INFINITY;
+                }
             }
-        } else {
+        }
+    };
+    const int chunks = (hi - lo + kChunk - 1) / kChunk;
+    uint4 raw[2][kLoads];
+    fetch(0, raw[0]);
+    if (chunks > 1) fetch(1, raw[1]);
+    if (tid == 0) s_count = 0;
+    float m = -INFINITY, sum = 0.0f, bound_value = -INFINITY;
+    uint64_t bound = 0;
+    for (int c0 = 0; c0 < chunks; c0 += 2) {
 #pragma unroll
-            for (int e = 0; e < kVec; ++e) v[i + e] = t + e < p.vocab ? static_cast<float>(x[t + e]) : -INFINITY;
+        for (int h = 0; h < 2; ++h) {
+            const int c = c0 + h;
+            if (c >= chunks) break;
+            float v[kItems];
+            unpack(c, raw[h], v);
+            if (c + 2 < chunks) fetch(c + 2, raw[h]);
+            float top = v[0];
+#pragma unroll
+            for (int i = 1; i < kItems; ++i) top = fmaxf(top, v[i]);
+            if (top > m) {
+                sum *= __expf(m - top);
+                m = top;
+            }
+            // a NaN or +inf logit makes the sum NaN, which kills the row
+            const float base = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+            for (int i = 0; i < kItems; ++i) sum += __expf(v[i] - base);   // a place past the slice adds 0
+            if (c == 0) {
+                const int full = min(kThreads, (hi - lo) / kVec) / 32;   // warps whose threads all have tokens
+                const bool bounded = full * 32 >= p.keep;
+                if (bounded && warp < full) {
+                    int first = 0;
+#pragma unroll
+                    for (int i = kItems - 1; i >= 0; --i) first = v[i] == top ? token(0, i) : first;
+                    uint32_t high = ordered_bits(top), low = ~static_cast<uint32_t>(first);
+                    const int rounds = (p.keep + full - 1) / full;
+                    uint32_t bh = 0, bl = 0;
+                    for (int r = 0; r < rounds; ++r) {
+                        bh = __reduce_max_sync(~0u, high);
+                        bl = __reduce_max_sync(~0u, high == bh ? low : 0u);
+                        if (high == bh && low == bl) high = low = 0;
+                    }
+                    if (lane == 0) s_bound[warp] = (static_cast<uint64_t>(bh) << 32) | bl;
+                }
+                __syncthreads();
+                if (bounded) {
+                    bound = s_bound[0];
+                    for (int w = 1; w < full; ++w) bound = s_bound[w] < bound ? s_bound[w] : bound;
+                    bound_value = from_ordered(static_cast<uint32_t>(bound >> 32));
+                }
+            }
+            if (top >= bound_value) {
+#pragma unroll
+                for (int i = 0; i < kItems; ++i) {
+                    const int t = token(c, i);
+                    if (v[i] >= bound_value && t < hi) {
+                        const uint64_t k = key(v[i], t);
+                        if (k >= bound) s_cand[atomicAdd(&s_count, 1)] = k;
+                    }
+                }
+            }
+            __syncthreads();
+            const int n = s_count;
+            __syncthreads();   // every thread has read the count before the next chunk adds to it
+            if (c + 1 < chunks && (c == 0 ? n > p.keep : n > kSoft)) {
+                const int left = cut(s_cand, &s_count, s_part, n, p.keep);
+                if (left == p.keep) {
+                    bound = s_cand[p.keep - 1];
+                    bound_value = from_ordered(static_cast<uint32_t>(bound >> 32));
+                }
+            }
         }
     }
-    float m = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < ITEMS; ++i) m = fmaxf(m, v[i]);
+    const int n = cut(s_cand, &s_count, s_part, s_count, p.keep);
+    uint64_t* out = p.keys + (static_cast<int64_t>(row) * p.slices + slice) * p.keep;
+    for (int i = tid; i < p.keep; i += kThreads) out[i] = i < n ? s_cand[i] : 0;
     float bm = m;
 #pragma unroll
     for (int o = 16; o; o >>= 1) bm = fmaxf(bm, __shfl_xor_sync(~0u, bm, o));
-    if (lane == 0) s_red[0][warp] = bm;
-    if (tid == 0) s_count = 0;
-    // the warp's r-th largest of its threads' maxima, taken out one by one
-    const int threads_used = min(kThreads, (p.vocab - base + kVec - 1) / kVec);
-    const int full = threads_used / 32;
-    const bool bounded = full * 32 >= p.keep;
-    if (bounded && warp < full) {
-        int first = 0;
-#pragma unroll
-        for (int i = ITEMS - 1; i >= 0; --i) first = v[i] == m ? token(i) : first;
-        uint32_t hi = ordered_bits(m), lo = ~static_cast<uint32_t>(first);
-        const int rounds = (p.keep + full - 1) / full;
-        uint32_t bh = 0, bl = 0;
-        for (int r = 0; r < rounds; ++r) {
-            bh = __reduce_max_sync(~0u, hi);
-            bl = __reduce_max_sync(~0u, hi == bh ? lo : 0u);
-            if (hi == bh && lo == bl) hi = lo = 0;
-        }
-        if (lane == 0) s_bound[warp] = (static_cast<uint64_t>(bh) << 32) | bl;
-    }
-    __syncthreads();
-    bm = s_red[0][0];
-#pragma unroll
-    for (int w = 1; w < kWarps; ++w) bm = fmaxf(bm, s_red[0][w]);
-    // sum of exp(v - bm); a NaN or +inf logit makes it NaN, which kills the row
-    float sum = 0.0f;
-    if (bm != -INFINITY) {
-#pragma unroll
-        for (int i = 0; i < ITEMS; ++i) sum += __expf(v[i] - bm);   // a place past the vocabulary adds 0
-    } else {
-#pragma unroll
-        for (int i = 0; i < ITEMS; ++i) sum += isnan(v[i]) ? v[i] : 0.0f;
-    }
+    sum *= m == -INFINITY ? 1.0f : __expf(m - bm);   // a thread that saw -inf only has 0, or NaN
 #pragma unroll
     for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-    if (lane == 0) s_red[1][warp] = sum;
-    uint64_t bound = 0;
-    if (bounded) {
-        bound = s_bound[0];
-        for (int w = 1; w < full; ++w) bound = s_bound[w] < bound ? s_bound[w] : bound;
+    if (lane == 0) {
+        s_max[warp] = bm;
+        s_sum[warp] = sum;
     }
-    auto collect = [&]() {
-        const float bound_value = bound ? from_ordered(static_cast<uint32_t>(bound >> 32)) : -INFINITY;
-#pragma unroll
-        for (int i = 0; i < ITEMS; ++i)
-            if (!(v[i] < bound_value) && token(i) < p.vocab) {
-                const uint64_t k = key(v[i], token(i));
-                if (k >= bound) {
-                    const int at = atomicAdd(&s_count, 1);
-                    if (at < kCand) s_cand[at] = k;
-                }
-            }
-    };
-    collect();
     __syncthreads();
-    if (s_count > kCand) {   // the same for every thread
-        // the largest bound that keep keys reach, one bit at a time
-        bound = 0;
-        for (int bit = 63; bit >= 0; --bit) {
-            const uint64_t tried = bound | (1ull << bit);
-            int n = 0;
-#pragma unroll
-            for (int i = 0; i < ITEMS; ++i) n += token(i) < p.vocab && key(v[i], token(i)) >= tried;
-            n = __reduce_add_sync(~0u, n);
-            __syncthreads();
-            if (lane == 0) s_bound[warp] = n;
-            __syncthreads();
-            n = 0;
-            for (int w = 0; w < kWarps; ++w) n += static_cast<int>(s_bound[w]);
-            if (n >= p.keep) bound = tried;
-        }
-        __syncthreads();
-        if (tid == 0) s_count = 0;
-        __syncthreads();
-        collect();
-        __syncthreads();
-    }
-    const int n = s_count;
-    uint64_t* out = p.keys + (static_cast<int64_t>(row) * p.slices + slice) * p.keep;
-    for (int i = tid; i < n; i += kThreads) {
-        const uint64_t k = s_cand[i];
-        int rank = 0;
-        for (int j = 0; j < n; ++j) rank += s_cand[j] > k;
-        if (rank < p.keep) out[rank] = k;
-    }
-    for (int i = n + tid; i < p.keep; i += kThreads) out[i] = 0;
     if (tid == 0) {
-        float total = 0.0f;
-        for (int w = 0; w < kWarps; ++w) total += s_red[1][w];
-        p.part[static_cast<int64_t>(row) * p.slices + slice] = make_float2(bm, total);
+        float all = s_max[0], total = 0.0f;
+        for (int w = 1; w < kWarps; ++w) all = fmaxf(all, s_max[w]);
+        for (int w = 0; w < kWarps; ++w) total += s_max[w] == -INFINITY ? s_sum[w] : s_sum[w] * __expf(s_max[w] - all);
+        p.part[static_cast<int64_t>(row) * p.slices + slice] = make_float2(all, total);
     }
 }
 
@@ -204,12 +264,17 @@ __device__ __forceinline__ void warp_merge(const uint64_t* lists, int n_lists, i
     const uint64_t bound = lo > hi ? lo : hi;
     int n = 0;
     const int total = n_lists * keep;
-    for (int i0 = 0; i0 < total; i0 += 32) {
-        const uint64_t k = i0 + lane < total ? lists[i0 + lane] : 0;
-        const bool in = k != 0 && k >= bound;
-        const uint32_t mask = __ballot_sync(~0u, in);
-        if (in) buf[n + __popc(mask & ((1u << lane) - 1))] = k;
-        n += __popc(mask);
+    for (int i0 = 0; i0 < total; i0 += 256) {   // eight loads in flight a lane
+        uint64_t k[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) k[u] = i0 + 32 * u + lane < total ? lists[i0 + 32 * u + lane] : 0;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const bool in = k[u] != 0 && k[u] >= bound;
+            const uint32_t mask = __ballot_sync(~0u, in);
+            if (in) buf[n + __popc(mask & ((1u << lane) - 1))] = k[u];
+            n += __popc(mask);
+        }
     }
     __syncwarp();
     for (int i = lane; i < n; i += 32) {
@@ -235,19 +300,22 @@ __global__ void beam_merge_kernel(const Params p, int buf_keys) {
     uint64_t* buf = s_final + p.beams * K + warp * buf_keys;
     for (int b = warp; b < p.beams; b += warps) {
         const int64_t row = static_cast<int64_t>(g) * p.beams + b;
+        const float prior = p.scores[row];
+        float2 part[kMaxSlices / 32];
         float m = -INFINITY;
-        for (int s = lane; s < p.slices; s += 32) m = fmaxf(m, p.part[row * p.slices + s].x);
+#pragma unroll
+        for (int s = 0; s < kMaxSlices / 32; ++s) {
+            part[s] = 32 * s + lane < p.slices ? p.part[row * p.slices + 32 * s + lane] : make_float2(-INFINITY, 0.0f);
+            m = fmaxf(m, part[s].x);
+        }
 #pragma unroll
         for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
         float sum = 0.0f;
-        for (int s = lane; s < p.slices; s += 32) {
-            const float2 v = p.part[row * p.slices + s];
-            sum += v.x == -INFINITY ? v.y : v.y * __expf(v.x - m);
-        }
+#pragma unroll
+        for (int s = 0; s < kMaxSlices / 32; ++s) sum += part[s].x == -INFINITY ? part[s].y : part[s].y * __expf(part[s].x - m);
 #pragma unroll
         for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
         const float lse = m + logf(sum);
-        const float prior = p.scores[row];
         uint64_t* list = s_list + b * K;
         // every continuation of a dead beam scores -inf: its tokens count in their own order
         const bool dead = !(fabsf(lse) < INFINITY) || isnan(prior) || prior == -INFINITY;
@@ -280,9 +348,9 @@ __global__ void beam_merge_kernel(const Params p, int buf_keys) {
     }
 }
 
-template <typename T, int ITEMS>
+template <typename T>
 static int launch(const Params& p, bool vec, cudaStream_t stream) {
-    auto scan = vec ? beam_scan_kernel<T, ITEMS, true> : beam_scan_kernel<T, ITEMS, false>;
+    auto scan = vec ? beam_scan_kernel<T, true> : beam_scan_kernel<T, false>;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(p.slices), static_cast<unsigned>(p.groups * p.beams));
     cfg.blockDim = dim3(kThreads);
@@ -318,7 +386,7 @@ extern "C" int bybycu_beam_select(const void* logits, int logits_dtype, int64_t 
     if (logits_dtype != BYBYCU_DT_F32 && logits_dtype != BYBYCU_DT_BF16)
         return set_error(BYBYCU_ERR_ARGS, "beam_select: logits must be F32 or BF16");
     if (groups < 0 || beams < 1 || beams > 64 || vocab < 1 || keep < 1 || keep > beam::kMaxKeep ||
-        keep > static_cast<int64_t>(beams) * vocab || vocab > beam::kThreads * 32 * beam::kMaxSlices)
+        keep > static_cast<int64_t>(beams) * vocab || vocab > (1 << 20))
         return set_error(BYBYCU_ERR_SHAPE, "beam_select: groups=%d beams=%d vocab=%d keep=%d", groups, beams, vocab, keep);
     if (static_cast<int64_t>(groups) * beams > 65535)
         return set_error(BYBYCU_ERR_SHAPE, "beam_select: more than 65535 rows (%d groups of %d beams)", groups, beams);
@@ -332,15 +400,16 @@ extern "C" int bybycu_beam_select(const void* logits, int logits_dtype, int64_t 
     DeviceInfo info;
     if (int rc = current_device_info(&info)) return rc;
     const int64_t rows = static_cast<int64_t>(groups) * beams;
-    // 32 logits a thread, or 8 where that would leave the card half empty
-    const bool small = rows * ceil_div(vocab, beam::kThreads * 32) < 2 * info.sm_count &&
-                       ceil_div(vocab, beam::kThreads * 8) <= beam::kMaxSlices;
+    // Slices of whole chunks: as many as fill the card's four blocks an SM about twice.
+    const int chunks = static_cast<int>(ceil_div(vocab, beam::kChunk));
+    const int wanted = static_cast<int>(std::min<int64_t>({chunks, beam::kMaxSlices, std::max<int64_t>(1, ceil_div(8 * info.sm_count, rows))}));
     beam::Params p{};
     p.x = logits;
     p.row_stride = row_stride;
     p.scores = scores;
     p.groups = groups; p.beams = beams; p.vocab = vocab; p.keep = keep;
-    p.slices = static_cast<int>(ceil_div(vocab, beam::kThreads * (small ? 8 : 32)));
+    p.slice_len = static_cast<int>(ceil_div(chunks, wanted)) * beam::kChunk;
+    p.slices = static_cast<int>(ceil_div(vocab, p.slice_len));
     p.out_scores = out_scores; p.out_beams = out_beams; p.out_tokens = out_tokens;
     const bool vec = kvc::aligned(logits, 16) && row_stride * esz % 16 == 0;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -352,8 +421,8 @@ extern "C" int bybycu_beam_select(const void* logits, int logits_dtype, int64_t 
     p.keys = static_cast<uint64_t*>(scratch);
     p.part = reinterpret_cast<float2*>(static_cast<char*>(scratch) + key_bytes);
     int rc;
-    if (logits_dtype == BYBYCU_DT_F32) rc = small ? beam::launch<float, 8>(p, vec, s) : beam::launch<float, 32>(p, vec, s);
-    else rc = small ? beam::launch<__nv_bfloat16, 8>(p, vec, s) : beam::launch<__nv_bfloat16, 32>(p, vec, s);
+    if (logits_dtype == BYBYCU_DT_F32) rc = beam::launch<float>(p, vec, s);
+    else rc = beam::launch<__nv_bfloat16>(p, vec, s);
     const cudaError_t fe = cudaFreeAsync(scratch, s);
     if (rc) return rc;
     if (fe != cudaSuccess) return cuda_fail(fe, "cudaFreeAsync(beam scratch)");

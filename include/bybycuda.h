@@ -413,7 +413,7 @@ BYBYCU_API int bybycu_copy_pages(void* k, void* v, int n_layers, int64_t layer_s
  * scores by the lower b, then the lower t.  A NaN sum (a row with no finite logit, with NaN or
  * with +inf) counts as -inf.  logits F32 or BF16 [groups * beams, vocab], rows row_stride elements
  * apart; scores fp32 [groups, beams]; the outputs [groups, keep].  1 <= keep <= 64, at most
- * beams * vocab; beams <= 64. */
+ * beams * vocab; beams <= 64, vocab <= 2^20, at most 65535 rows. */
 BYBYCU_API int bybycu_beam_select(const void* logits, int logits_dtype, int64_t row_stride, const float* scores,
                                   int groups, int beams, int vocab, int keep, float* out_scores,
                                   int32_t* out_beams, int32_t* out_tokens, void* stream);
