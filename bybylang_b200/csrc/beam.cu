@@ -21,20 +21,19 @@ static int scratch_pool(int device, cudaMemPool_t* pool);
 namespace beam {
 
 constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
 constexpr int kMaxKeep = 64;
-constexpr int kMaxSlices = 128;
-constexpr int kItems = 8;                     // logits of a thread in one chunk
-constexpr int kChunk = kThreads * kItems;     // 2048
-constexpr int kSoft = 256;                    // candidates above which they are cut down to the best `keep`
-constexpr int kCand = kSoft + kChunk;         // so that a whole chunk always finds room
-constexpr int kRanked = 512;                  // candidates that are ranked against each other; more are bisected first
-static_assert(kSoft >= 2 * kMaxKeep, "a cut has to make room");
+constexpr int kMaxSlices = 32;
+constexpr int kItems = 8;                       // logits of a lane in one chunk
+constexpr int kChunk = 32 * kItems;             // of a warp
+constexpr int kSoft = 2 * kMaxKeep;             // candidates above which a warp cuts them down to the best `keep`
+constexpr int kCand = kSoft + kChunk;           // so that a whole chunk always finds room
 
 struct Params {
     const void* x;
     int64_t row_stride;
     const float* scores;
-    int groups, beams, vocab, keep, slices, slice_len;   // slice_len: a multiple of kChunk
+    int groups, beams, vocab, keep, slices, slice_len;   // slice_len: a multiple of kWarps * kChunk
     float2* part;        // [rows][slices] maximum and sum of a slice
     uint64_t* keys;      // [rows][slices][keep] the slice's best, best first; 0 = none
     float* out_scores;
@@ -42,6 +41,12 @@ struct Params {
     int32_t* out_tokens;
 };
 
+constexpr float kLog2e = 1.4426950408889634f;
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 __device__ __forceinline__ uint32_t ordered_bits(float v) {
     const uint32_t u = __float_as_uint(v + 0.0f);   // -0 orders as +0
     return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
@@ -50,79 +55,109 @@ __device__ __forceinline__ float from_ordered(uint32_t u) {
     return __uint_as_float(u ^ ((u >> 31) ? 0x80000000u : 0xffffffffu));
 }
 
-// Cuts the n candidates of s_cand down to the best `keep`, sorted; the new count, the same for
-// every thread.  Ranks by counting; more than kRanked are first bisected down to exactly `keep`,
-// one key bit at a time.
-__device__ __forceinline__ int cut(uint64_t* s_cand, int* s_count, int* s_part, int n, int keep) {
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    constexpr int kWarps = kThreads / 32, kMine = (kCand + kThreads - 1) / kThreads;
-    if (n > kRanked) {
-        uint64_t bound = 0;
-        for (int bit = 63; bit >= 0; --bit) {
-            const uint64_t tried = bound | (1ull << bit);
-            int c = 0;
-            for (int i = tid; i < n; i += kThreads) c += s_cand[i] >= tried;
-            c = __reduce_add_sync(~0u, c);
-            if (lane == 0) s_part[warp] = c;
-            __syncthreads();
-            c = 0;
-            for (int w = 0; w < kWarps; ++w) c += s_part[w];
-            __syncthreads();
-            if (c >= keep) bound = tried;
-        }
-        uint64_t mine[kMine];
-#pragma unroll
-        for (int i = 0; i < kMine; ++i) mine[i] = i * kThreads + tid < n ? s_cand[i * kThreads + tid] : 0;
-        if (tid == 0) *s_count = 0;
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < kMine; ++i)
-            if (mine[i] >= bound && mine[i] != 0) s_cand[atomicAdd(s_count, 1)] = mine[i];
-        __syncthreads();
-        n = *s_count;
+// Writes the best `keep` of a warp's n candidates to `list`, sorted, by counting for each the
+// larger ones; how many there are.
+__device__ __forceinline__ int warp_best(const uint64_t* cand, int n, int keep, uint64_t* list, int lane) {
+    __syncwarp();
+    for (int i = lane; i < n; i += 32) {
+        const uint64_t k = cand[i];
+        int rank = 0;
+#pragma unroll 4
+        for (int j = 0; j < n; ++j) rank += cand[j] > k;
+        if (rank < keep) list[rank] = k;
     }
-    uint64_t k[kRanked / kThreads];
-    int rank[kRanked / kThreads] = {};
-#pragma unroll
-    for (int i = 0; i < kRanked / kThreads; ++i) k[i] = i * kThreads + tid < n ? s_cand[i * kThreads + tid] : 0;
-    for (int j = 0; j < n; ++j) {
-        const uint64_t o = s_cand[j];
-#pragma unroll
-        for (int i = 0; i < kRanked / kThreads; ++i) rank[i] += o > k[i];
-    }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kRanked / kThreads; ++i)
-        if (i * kThreads + tid < n && rank[i] < keep) s_cand[rank[i]] = k[i];
-    n = min(n, keep);
-    if (tid == 0) *s_count = n;
-    __syncthreads();
-    return n;
+    __syncwarp();
+    return min(n, keep);
 }
 
-// One slice of one row, chunk by chunk.  A logit is a candidate when it is not below the bound,
-// the keep-th best so far; the first chunk has a bound to start from: every warp takes the r-th
-// largest of its threads' own maxima, r = ceil(keep / warps), and at least keep keys are not below
-// the smallest of these.  For logits in no particular order some 2 * keep elements of the first
-// chunk and keep / c of the c-th become candidates.
+// The `keep` largest of n_lists sorted lists of `keep` keys each, by one warp, into out[keep]
+// (sorted, 0 where there are fewer).  Every list's e-th entry, e = ceil(keep / n_lists), bounds
+// the result from below through the smallest of them, as does any list's last entry.
+__device__ __forceinline__ void warp_merge(const uint64_t* lists, int n_lists, int keep, uint64_t* buf, uint64_t* out,
+                                           int lane) {
+    const int e = (keep + n_lists - 1) / n_lists - 1;
+    uint64_t lo = ~0ull, hi = 0;
+    for (int l = lane; l < n_lists; l += 32) {
+        const uint64_t a = lists[l * keep + e], z = lists[l * keep + keep - 1];
+        lo = a < lo ? a : lo;
+        hi = z > hi ? z : hi;
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        const uint64_t a = __shfl_xor_sync(~0u, lo, o), z = __shfl_xor_sync(~0u, hi, o);
+        lo = a < lo ? a : lo;
+        hi = z > hi ? z : hi;
+    }
+    uint64_t bound = lo > hi ? lo : hi;
+    if (n_lists > 2 * keep) {   // of many short lists the keep-th largest head bounds better
+        uint64_t head[2];   // up to 64 lists
+#pragma unroll
+        for (int i = 0; i < 2; ++i) head[i] = 32 * i + lane < n_lists ? lists[(32 * i + lane) * keep] : 0;
+        uint64_t kth = 0;
+        for (int r = 0; r < keep; ++r) {
+            const uint64_t top = head[0] > head[1] ? head[0] : head[1];
+            const uint32_t bh = __reduce_max_sync(~0u, static_cast<uint32_t>(top >> 32));
+            const uint32_t bl = __reduce_max_sync(~0u, static_cast<uint32_t>(top >> 32) == bh ? static_cast<uint32_t>(top) : 0u);
+            kth = (static_cast<uint64_t>(bh) << 32) | bl;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) head[i] = head[i] == kth ? 0 : head[i];
+        }
+        bound = kth > bound ? kth : bound;
+    }
+    int n = 0;
+    const int total = n_lists * keep;
+    for (int i0 = 0; i0 < total; i0 += 256) {   // eight loads in flight a lane
+        uint64_t k[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) k[u] = i0 + 32 * u + lane < total ? lists[i0 + 32 * u + lane] : 0;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const bool in = k[u] != 0 && k[u] >= bound;
+            const uint32_t mask = __ballot_sync(~0u, in);
+            if (in) buf[n + __popc(mask & ((1u << lane) - 1))] = k[u];
+            n += __popc(mask);
+        }
+    }
+    __syncwarp();
+    for (int i = lane; i < n; i += 32) {
+        const uint64_t k = buf[i];
+        int rank = 0;
+#pragma unroll 4
+        for (int j = 0; j < n; ++j) rank += buf[j] > k;
+        if (rank < keep) out[rank] = k;
+    }
+    for (int i = n + lane; i < keep; i += 32) out[i] = 0;
+    __syncwarp();
+}
+
+// One slice of one row.  Each warp walks its own chunks with its own candidates: a logit is one
+// when it is not below the warp's bound.  The first bound comes from all warps' first chunks: each
+// takes the r-th largest of its lanes' maxima, r = ceil(keep / warps), and at least keep keys are
+// not below the smallest of these.  After 2, 4, 8, 16 and 32 chunks the same with the r-th best
+// candidates, so that for logits in no particular order some 2 * keep / c elements of the c-th
+// chunks become candidates.  A warp that has more than kSoft cuts them down to its best keep.
+// Bound by the row's stream from HBM in the end; instructions a logit are what it takes to get
+// there (256 rows of 128256 bf16, 66 MB: block-wide bounds met at a barrier every 2048 logits 61 us,
+// a warp's bound from its own 256 logits 80 us).
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kThreads, 4) beam_scan_kernel(const Params p) {
-    __shared__ uint64_t s_cand[kCand];
-    __shared__ uint64_t s_bound[kThreads / 32];
-    __shared__ float s_max[kThreads / 32], s_sum[kThreads / 32];
-    __shared__ int s_part[kThreads / 32];
-    __shared__ int s_count;
+    __shared__ uint64_t s_cand[kWarps * kCand];
+    __shared__ uint64_t s_list[kWarps * kMaxKeep];
+    __shared__ uint64_t s_bound[kWarps];
+    __shared__ float s_max[kWarps], s_sum[kWarps];
+    __shared__ int s_count[kWarps];
     pdl_launch_dependents();
     pdl_wait();
     constexpr int kVec = VEC ? 16 / static_cast<int>(sizeof(T)) : 1, kLoads = kItems / kVec;
-    constexpr int kWarps = kThreads / 32;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int row = blockIdx.y, slice = blockIdx.x;
     const int lo = slice * p.slice_len, hi = min(p.vocab, lo + p.slice_len);
     const T* x = static_cast<const T*>(p.x) + row * p.row_stride;
-    // a thread's tokens of a chunk ascend with i
-    auto token = [&](int c, int i) { return lo + c * kChunk + (i / kVec * kThreads + tid) * kVec + i % kVec; };
-    auto key = [&](float v, int t) { return (static_cast<uint64_t>(ordered_bits(v)) << 32) | ~static_cast<uint32_t>(t); };
+    uint64_t* cand = s_cand + warp * kCand;
+    uint64_t* list = s_list + warp * p.keep;
+    int* count = s_count + warp;
+    // a lane's tokens of the warp's c-th chunk ascend with i
+    auto token = [&](int c, int i) { return lo + (c * kWarps + warp) * kChunk + (i / kVec * 32 + lane) * kVec + i % kVec; };
     auto fetch = [&](int c, uint4 (&raw)[kLoads]) {   // whole vectors only; the ragged end is read by itself
         if constexpr (VEC) {
 #pragma unroll
@@ -149,11 +184,26 @@ __global__ void __launch_bounds__(kThreads, 4) beam_scan_kernel(const Params p) 
             }
         }
     };
-    const int chunks = (hi - lo + kChunk - 1) / kChunk;
+    const int left = hi - lo - warp * kChunk;   // of this warp's part
+    const int chunks = left > 0 ? (left + kWarps * kChunk - 1) / (kWarps * kChunk) : 0;
     uint4 raw[2][kLoads];
-    fetch(0, raw[0]);
-    if (chunks > 1) fetch(1, raw[1]);
-    if (tid == 0) s_count = 0;
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+        if (c < chunks) fetch(c, raw[c]);
+    if (lane == 0) *count = 0;
+    __syncwarp();
+    const bool bounded = hi - lo >= kWarps * kChunk;   // every lane of every warp has a whole first chunk
+    const int share = (p.keep + kWarps - 1) / kWarps;
+    // the smallest of the warps' keys; every warp calls
+    auto join_bounds = [&](uint64_t mine) {
+        if (lane == 0) s_bound[warp] = mine;
+        __syncthreads();
+        uint64_t least = s_bound[0];
+        for (int w = 1; w < kWarps; ++w) least = s_bound[w] < least ? s_bound[w] : least;
+        __syncthreads();
+        return least;
+    };
+    const int common = (hi - lo) / (kWarps * kChunk);   // chunks that every warp has in whole
     float m = -INFINITY, sum = 0.0f, bound_value = -INFINITY;
     uint64_t bound = 0;
     for (int c0 = 0; c0 < chunks; c0 += 2) {
@@ -168,66 +218,71 @@ __global__ void __launch_bounds__(kThreads, 4) beam_scan_kernel(const Params p) 
 #pragma unroll
             for (int i = 1; i < kItems; ++i) top = fmaxf(top, v[i]);
             if (top > m) {
-                sum *= __expf(m - top);
+                sum *= ex2((m - top) * kLog2e);
                 m = top;
             }
             // a NaN or +inf logit makes the sum NaN, which kills the row
-            const float base = m == -INFINITY ? 0.0f : m;
+            const float off = m == -INFINITY ? 0.0f : -m * kLog2e;
 #pragma unroll
-            for (int i = 0; i < kItems; ++i) sum += __expf(v[i] - base);   // a place past the slice adds 0
-            if (c == 0) {
-                const int full = min(kThreads, (hi - lo) / kVec) / 32;   // warps whose threads all have tokens
-                const bool bounded = full * 32 >= p.keep;
-                if (bounded && warp < full) {
-                    int first = 0;
+            for (int i = 0; i < kItems; ++i) sum += ex2(fmaf(v[i], kLog2e, off));   // a place past the slice adds 0
+            if (c == 0 && left >= 32 * kVec && (bounded || p.keep <= 32)) {
+                int first = 0;
 #pragma unroll
-                    for (int i = kItems - 1; i >= 0; --i) first = v[i] == top ? token(0, i) : first;
-                    uint32_t high = ordered_bits(top), low = ~static_cast<uint32_t>(first);
-                    const int rounds = (p.keep + full - 1) / full;
-                    uint32_t bh = 0, bl = 0;
-                    for (int r = 0; r < rounds; ++r) {
-                        bh = __reduce_max_sync(~0u, high);
-                        bl = __reduce_max_sync(~0u, high == bh ? low : 0u);
-                        if (high == bh && low == bl) high = low = 0;
-                    }
-                    if (lane == 0) s_bound[warp] = (static_cast<uint64_t>(bh) << 32) | bl;
+                for (int i = kItems - 1; i >= 0; --i) first = v[i] == top ? token(0, i) : first;
+                uint32_t high = ordered_bits(top), low = ~static_cast<uint32_t>(first), bh = 0, bl = 0;
+                const int rounds = bounded ? share : p.keep;   // a short slice: each warp for itself
+                for (int r = 0; r < rounds; ++r) {   // the maxima, taken out one by one
+                    bh = __reduce_max_sync(~0u, high);
+                    bl = __reduce_max_sync(~0u, high == bh ? low : 0u);
+                    if (high == bh && low == bl) high = low = 0;
                 }
-                __syncthreads();
-                if (bounded) {
-                    bound = s_bound[0];
-                    for (int w = 1; w < full; ++w) bound = s_bound[w] < bound ? s_bound[w] : bound;
-                    bound_value = from_ordered(static_cast<uint32_t>(bound >> 32));
-                }
+                bound = (static_cast<uint64_t>(bh) << 32) | bl;
+                if (bounded) bound = join_bounds(bound);
+                bound_value = from_ordered(static_cast<uint32_t>(bound >> 32));
             }
-            if (top >= bound_value) {
+            if (__any_sync(~0u, top >= bound_value)) {
+                uint32_t some = 0;
 #pragma unroll
-                for (int i = 0; i < kItems; ++i) {
-                    const int t = token(c, i);
-                    if (v[i] >= bound_value && t < hi) {
-                        const uint64_t k = key(v[i], t);
-                        if (k >= bound) s_cand[atomicAdd(&s_count, 1)] = k;
+                for (int i = 0; i < kItems; ++i) some |= v[i] >= bound_value && token(c, i) < hi ? 1u << i : 0u;
+                while (some) {   // few: read again rather than kept in reach of an index
+                    const int t = token(c, __ffs(some) - 1);
+                    const uint64_t k = (static_cast<uint64_t>(ordered_bits(static_cast<float>(x[t]))) << 32) | ~static_cast<uint32_t>(t);
+                    if (k >= bound) cand[atomicAdd(count, 1)] = k;
+                    some &= some - 1;
+                }
+                __syncwarp();
+                const int n = *count;
+                if (c + 1 < chunks && n > kSoft) {
+                    const int now = warp_best(cand, n, p.keep, list, lane);
+                    for (int i = lane; i < now; i += 32) cand[i] = list[i];
+                    if (lane == 0) *count = now;
+                    if (now == p.keep) {
+                        bound = list[p.keep - 1];
+                        bound_value = from_ordered(static_cast<uint32_t>(bound >> 32));
                     }
                 }
+                __syncwarp();
             }
-            __syncthreads();
-            const int n = s_count;
-            __syncthreads();   // every thread has read the count before the next chunk adds to it
-            if (c + 1 < chunks && (c == 0 ? n > p.keep : n > kSoft)) {
-                const int left = cut(s_cand, &s_count, s_part, n, p.keep);
-                if (left == p.keep) {
-                    bound = s_cand[p.keep - 1];
+            if (bounded && c + 1 < common && (c == 1 || c == 3 || c == 7 || c == 15 || c == 31)) {
+                // the bound follows: the share-th best of each warp so far
+                const int now = warp_best(cand, *count, p.keep, list, lane);
+                for (int i = lane; i < now; i += 32) cand[i] = list[i];
+                if (lane == 0) *count = now;
+                __syncwarp();
+                const uint64_t joint = join_bounds(now >= share ? list[share - 1] : 0);
+                if (joint > bound) {
+                    bound = joint;
                     bound_value = from_ordered(static_cast<uint32_t>(bound >> 32));
                 }
             }
         }
     }
-    const int n = cut(s_cand, &s_count, s_part, s_count, p.keep);
-    uint64_t* out = p.keys + (static_cast<int64_t>(row) * p.slices + slice) * p.keep;
-    for (int i = tid; i < p.keep; i += kThreads) out[i] = i < n ? s_cand[i] : 0;
+    const int n = warp_best(cand, *count, p.keep, list, lane);
+    for (int i = n + lane; i < p.keep; i += 32) list[i] = 0;
     float bm = m;
 #pragma unroll
     for (int o = 16; o; o >>= 1) bm = fmaxf(bm, __shfl_xor_sync(~0u, bm, o));
-    sum *= m == -INFINITY ? 1.0f : __expf(m - bm);   // a thread that saw -inf only has 0, or NaN
+    sum *= m == -INFINITY ? 1.0f : ex2((m - bm) * kLog2e);   // a lane that saw -inf only has 0, or NaN
 #pragma unroll
     for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
     if (lane == 0) {
@@ -235,56 +290,15 @@ __global__ void __launch_bounds__(kThreads, 4) beam_scan_kernel(const Params p) 
         s_sum[warp] = sum;
     }
     __syncthreads();
-    if (tid == 0) {
+    const int64_t at = static_cast<int64_t>(row) * p.slices + slice;
+    if (warp == 0) {
+        warp_merge(s_list, kWarps, p.keep, s_cand, p.keys + at * p.keep, lane);   // the warps' candidates are done with
+    } else if (threadIdx.x == 32) {
         float all = s_max[0], total = 0.0f;
         for (int w = 1; w < kWarps; ++w) all = fmaxf(all, s_max[w]);
-        for (int w = 0; w < kWarps; ++w) total += s_max[w] == -INFINITY ? s_sum[w] : s_sum[w] * __expf(s_max[w] - all);
-        p.part[static_cast<int64_t>(row) * p.slices + slice] = make_float2(all, total);
+        for (int w = 0; w < kWarps; ++w) total += s_max[w] == -INFINITY ? s_sum[w] : s_sum[w] * ex2((s_max[w] - all) * kLog2e);
+        p.part[at] = make_float2(all, total);
     }
-}
-
-// The `keep` largest of n_lists sorted lists of `keep` keys each, by one warp, into out[keep]
-// (sorted, 0 where there are fewer).  Every list's e-th entry, e = ceil(keep / n_lists), bounds
-// the result from below through the smallest of them, as does any list's last entry.
-__device__ __forceinline__ void warp_merge(const uint64_t* lists, int n_lists, int keep, uint64_t* buf, uint64_t* out,
-                                           int lane) {
-    const int e = (keep + n_lists - 1) / n_lists - 1;
-    uint64_t lo = ~0ull, hi = 0;
-    for (int l = lane; l < n_lists; l += 32) {
-        const uint64_t a = lists[l * keep + e], z = lists[l * keep + keep - 1];
-        lo = a < lo ? a : lo;
-        hi = z > hi ? z : hi;
-    }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-        const uint64_t a = __shfl_xor_sync(~0u, lo, o), z = __shfl_xor_sync(~0u, hi, o);
-        lo = a < lo ? a : lo;
-        hi = z > hi ? z : hi;
-    }
-    const uint64_t bound = lo > hi ? lo : hi;
-    int n = 0;
-    const int total = n_lists * keep;
-    for (int i0 = 0; i0 < total; i0 += 256) {   // eight loads in flight a lane
-        uint64_t k[8];
-#pragma unroll
-        for (int u = 0; u < 8; ++u) k[u] = i0 + 32 * u + lane < total ? lists[i0 + 32 * u + lane] : 0;
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
-            const bool in = k[u] != 0 && k[u] >= bound;
-            const uint32_t mask = __ballot_sync(~0u, in);
-            if (in) buf[n + __popc(mask & ((1u << lane) - 1))] = k[u];
-            n += __popc(mask);
-        }
-    }
-    __syncwarp();
-    for (int i = lane; i < n; i += 32) {
-        const uint64_t k = buf[i];
-        int rank = 0;
-        for (int j = 0; j < n; ++j) rank += buf[j] > k;
-        if (rank < keep) out[rank] = k;
-    }
-    for (int i = n + lane; i < keep; i += 32) out[i] = 0;
-    __syncwarp();
 }
 
 // One block per group: each warp joins the slices of its beams, then warp 0 the beams.
@@ -301,18 +315,11 @@ __global__ void beam_merge_kernel(const Params p, int buf_keys) {
     for (int b = warp; b < p.beams; b += warps) {
         const int64_t row = static_cast<int64_t>(g) * p.beams + b;
         const float prior = p.scores[row];
-        float2 part[kMaxSlices / 32];
-        float m = -INFINITY;
-#pragma unroll
-        for (int s = 0; s < kMaxSlices / 32; ++s) {
-            part[s] = 32 * s + lane < p.slices ? p.part[row * p.slices + 32 * s + lane] : make_float2(-INFINITY, 0.0f);
-            m = fmaxf(m, part[s].x);
-        }
+        const float2 part = lane < p.slices ? p.part[row * p.slices + lane] : make_float2(-INFINITY, 0.0f);
+        float m = part.x;
 #pragma unroll
         for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
-        float sum = 0.0f;
-#pragma unroll
-        for (int s = 0; s < kMaxSlices / 32; ++s) sum += part[s].x == -INFINITY ? part[s].y : part[s].y * __expf(part[s].x - m);
+        float sum = part.x == -INFINITY ? part.y : part.y * ex2((part.x - m) * kLog2e);
 #pragma unroll
         for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
         const float lse = m + logf(sum);
@@ -400,15 +407,18 @@ extern "C" int bybycu_beam_select(const void* logits, int logits_dtype, int64_t 
     DeviceInfo info;
     if (int rc = current_device_info(&info)) return rc;
     const int64_t rows = static_cast<int64_t>(groups) * beams;
-    // Slices of whole chunks: as many as fill the card's four blocks an SM about twice.
-    const int chunks = static_cast<int>(ceil_div(vocab, beam::kChunk));
-    const int wanted = static_cast<int>(std::min<int64_t>({chunks, beam::kMaxSlices, std::max<int64_t>(1, ceil_div(8 * info.sm_count, rows))}));
+    // Slices of whole chunks: two blocks an SM or a few more (1, 2, 4 times as many: 48, 53, 56 us at
+    // 256 rows of 128256 bf16), but no more than a warp
+    // of the second kernel joins at once.
+    constexpr int kPiece = beam::kWarps * beam::kChunk;
+    const int chunks = static_cast<int>(ceil_div(vocab, kPiece));
+    const int wanted = static_cast<int>(std::min<int64_t>({chunks, beam::kMaxSlices, std::max<int64_t>(1, ceil_div(2 * info.sm_count, rows))}));
     beam::Params p{};
     p.x = logits;
     p.row_stride = row_stride;
     p.scores = scores;
     p.groups = groups; p.beams = beams; p.vocab = vocab; p.keep = keep;
-    p.slice_len = static_cast<int>(ceil_div(chunks, wanted)) * beam::kChunk;
+    p.slice_len = static_cast<int>(ceil_div(chunks, wanted)) * kPiece;
     p.slices = static_cast<int>(ceil_div(vocab, p.slice_len));
     p.out_scores = out_scores; p.out_beams = out_beams; p.out_tokens = out_tokens;
     const bool vec = kvc::aligned(logits, 16) && row_stride * esz % 16 == 0;

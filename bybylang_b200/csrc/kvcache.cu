@@ -175,19 +175,22 @@ static int launch_rope(const Cache& c, const RopeParams& p, bool interleaved, bo
 // Each block moves one piece of one page of one layer of K or V.  The pairs ride in the launch's
 // parameters, so a call needs no copy to the device and keeps nothing alive after it returns.
 // ---------------------------------------------------------------------------------------
-constexpr int kCopyPairs = 1000;       // pairs of one launch: 8000 bytes of parameters
+constexpr int kCopyPairs = 1000;       // pairs of one launch: 8000 bytes of parameters,
+constexpr int kCopyFew = 56;           // or 448 where there are few (the launch copies them all)
 constexpr int kCopyThreads = 256;
 constexpr int kCopyUnroll = 4;         // 16-byte loads in flight per thread
 constexpr int kCopyPiece = kCopyThreads * kCopyUnroll * 16;   // 16 KiB
 
+template <int N>
 struct CopyParams {
     char* base[2];
     int64_t layer_stride, page_stride, page_bytes;
     int32_t pieces, n_tensors, n_layers;
-    int32_t pairs[2 * kCopyPairs];
+    int32_t pairs[2 * N];
 };
 
-__global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(const __grid_constant__ CopyParams p) {
+template <int N>
+__global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(const __grid_constant__ CopyParams<N> p) {
     pdl_launch_dependents();
     pdl_wait();
     const int pair = blockIdx.x / p.pieces, piece = blockIdx.x % p.pieces;
@@ -203,6 +206,39 @@ __global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(const __grid_c
 #pragma unroll
     for (int u = 0; u < kCopyUnroll; ++u)
         if (i0 + u * kCopyThreads < n) __stcs(dst + i0 + u * kCopyThreads, x[u]);
+}
+
+template <int N>
+static int launch_copy(CopyParams<N>& p, const int32_t* pairs, int n, cudaStream_t stream) {
+    std::copy(pairs, pairs + 2 * n, p.pairs);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(n * p.pieces), static_cast<unsigned>(p.n_layers), p.n_tensors);
+    cfg.blockDim = dim3(kCopyThreads);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    BYBYCU_CUDA_TRY(cudaLaunchKernelEx(&cfg, copy_pages_kernel<N>, p));
+    return BYBYCU_OK;
+}
+
+template <int N>
+static int copy_all(void* k, void* v, int n_layers, int64_t layer_stride, int64_t page_stride, int64_t page_bytes,
+                    int pieces, const int32_t* pairs, int n_pairs, cudaStream_t stream) {
+    CopyParams<N> p;
+    p.base[0] = static_cast<char*>(k);
+    p.base[1] = static_cast<char*>(v);
+    p.layer_stride = layer_stride;
+    p.page_stride = page_stride;
+    p.page_bytes = page_bytes;
+    p.pieces = pieces;
+    p.n_layers = n_layers;
+    p.n_tensors = v ? 2 : 1;
+    for (int at = 0; at < n_pairs; at += N)
+        if (int rc = launch_copy(p, pairs + 2 * at, std::min(N, n_pairs - at), stream)) return rc;
+    return BYBYCU_OK;
 }
 
 }  // namespace kvc
@@ -275,32 +311,11 @@ int bybycu_copy_pages(void* k, void* v, int n_layers, int64_t layer_stride, int6
         role[a] |= 1;
         role[b] |= 2;
     }
-    kvc::CopyParams p;
-    p.base[0] = static_cast<char*>(k);
-    p.base[1] = static_cast<char*>(v);
-    p.layer_stride = layer_stride;
-    p.page_stride = page_stride;
-    p.page_bytes = page_bytes;
     const int64_t pieces = ceil_div(page_bytes, kvc::kCopyPiece);
     if (pieces > (1 << 20)) return set_error(BYBYCU_ERR_SHAPE, "copy_pages: pages of %lld bytes", static_cast<long long>(page_bytes));
-    p.pieces = static_cast<int32_t>(pieces);
-    p.n_layers = n_layers;
-    p.n_tensors = v ? 2 : 1;
-    for (int at = 0; at < n_pairs; at += kvc::kCopyPairs) {
-        const int n = std::min(kvc::kCopyPairs, n_pairs - at);
-        std::copy(pairs + 2 * at, pairs + 2 * (at + n), p.pairs);
-        cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3(static_cast<unsigned>(n * pieces), static_cast<unsigned>(n_layers), p.n_tensors);
-        cfg.blockDim = dim3(kvc::kCopyThreads);
-        cfg.stream = static_cast<cudaStream_t>(stream);
-        cudaLaunchAttribute attr[1];
-        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[0].val.programmaticStreamSerializationAllowed = 1;
-        cfg.attrs = attr;
-        cfg.numAttrs = 1;
-        BYBYCU_CUDA_TRY(cudaLaunchKernelEx(&cfg, kvc::copy_pages_kernel, p));
-    }
-    return BYBYCU_OK;
+    auto all = n_pairs <= kvc::kCopyFew ? kvc::copy_all<kvc::kCopyFew> : kvc::copy_all<kvc::kCopyPairs>;
+    return all(k, v, n_layers, layer_stride, page_stride, page_bytes, static_cast<int>(pieces), pairs, n_pairs,
+               static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

@@ -22,49 +22,91 @@ from __future__ import annotations
 import ctypes as C
 import heapq
 import math
+import struct
 
 from . import _lib
 from ._lib import BybyCudaError, check, load
-from .gpubackend import _dtype_code, _ptr, _stream_ptr
+from .gpubackend import _dtype_code
+
+# A decode step makes several of these calls a layer, so what a call costs the host counts: the
+# argument structs of include/bybycuda.h are packed in one go (bybycu_paged_kv, bybycu_rope,
+# bybycu_attention, field by field), and passed as bytes.
+_KV = struct.Struct("=QQqqqQqQQ8i").pack
+_ROPE = struct.Struct("=QQQQ8qQQ4ifi").pack
+_ATTENTION = struct.Struct("=QQ4qQQ6i2f").pack
+_calls: dict = {}
+
+
+def _call(name: str):
+    fn = _calls.get(name)
+    if fn is None:
+        fn = load()[name]     # a handle of its own: raw pointers and bytes for the structs
+        fn.argtypes = [C.c_void_p if a not in (C.c_int, C.c_int64) else a for a in _lib.SIGNATURES[name]]
+        fn.restype = C.c_int
+        _calls[name] = fn
+    return fn
 
 
 def _refuse(code: int, message: str):
     raise BybyCudaError(code, message)
 
 
-def _paged(op: str, n_tokens: int, k_cache, v_cache, page_table, q_start, kv_lens) -> "_lib.PagedKv":
+def _stream(op: str, device: int, stream) -> int:
+    """The raw stream of a call on `device`, which has to be the current one."""
+    import torch
+    if stream is not None:
+        return stream.cuda_stream
+    if torch._C._cuda_getDevice() != device:
+        _refuse(_lib.ERR_ARGS, f"{op}: the tensors are on cuda:{device}, the current device is cuda:{torch.cuda.current_device()}")
+    return torch._C._cuda_getCurrentRawStream(device)
+
+
+def _paged(op: str, n_tokens: int, k_cache, v_cache, page_table, q_start, kv_lens):
+    """The packed bybycu_paged_kv and (device, sequences, kv heads, head dim) of a call's cache and batch."""
     import torch
     if k_cache.dim() != 4 or k_cache.dtype != torch.bfloat16 or v_cache.dtype != torch.bfloat16:
         _refuse(_lib.ERR_ARGS, f"{op}: caches must be bfloat16 [pages, kv heads, page size, head dim]")
-    n_pages, heads, page, dim = k_cache.shape
-    sp, sh, st, sd = k_cache.stride()
-    if v_cache.shape != k_cache.shape or v_cache.stride() != (sp, sh, st, sd) or sd != 1:
+    shape, strides = k_cache.shape, k_cache.stride()
+    n_pages, heads, page, dim = shape
+    if v_cache.shape != shape or v_cache.stride() != strides or strides[3] != 1:
         _refuse(_lib.ERR_ARGS, f"{op}: the caches must share shape and strides, the last dimension dense")
     if page_table.dim() != 2 or page_table.dtype != torch.int32 or q_start.dtype != torch.int32 or kv_lens.dtype != torch.int32:
         _refuse(_lib.ERR_ARGS, f"{op}: page_table [sequences, pages], q_start and kv_lens must be int32")
     n_seqs, max_pages = page_table.shape
     if q_start.numel() != n_seqs + 1 or kv_lens.numel() != n_seqs:
         _refuse(_lib.ERR_SHAPE, f"{op}: {n_seqs} sequences need {n_seqs + 1} starts and {n_seqs} lengths")
-    if not q_start.is_contiguous() or not kv_lens.is_contiguous() or (max_pages > 1 and page_table.stride(1) != 1):
+    table_stride, one = page_table.stride()
+    if not q_start.is_contiguous() or not kv_lens.is_contiguous() or (max_pages > 1 and one != 1):
         _refuse(_lib.ERR_ARGS, f"{op}: page_table rows, q_start and kv_lens must be contiguous")
-    for t in (k_cache, v_cache, page_table, q_start, kv_lens):
-        if not t.is_cuda:
-            _refuse(_lib.ERR_ARGS, f"{op}: every tensor must be on the device")
-    table_stride = page_table.stride(0) if n_seqs > 1 else max_pages
-    return _lib.PagedKv(k_cache.data_ptr(), v_cache.data_ptr(), sp, sh, st, page_table.data_ptr(), table_stride,
-                        q_start.data_ptr(), kv_lens.data_ptr(), n_pages, page, heads, dim, max_pages, n_seqs, n_tokens, 0)
+    dev = k_cache.get_device()
+    if dev < 0 or v_cache.get_device() != dev or page_table.get_device() != dev or q_start.get_device() != dev or \
+            kv_lens.get_device() != dev:
+        _refuse(_lib.ERR_ARGS, f"{op}: every tensor must be on the device")
+    if n_seqs <= 1:
+        table_stride = max_pages
+    return _KV(k_cache.data_ptr(), v_cache.data_ptr(), strides[0], strides[1], strides[2], page_table.data_ptr(), table_stride,
+               q_start.data_ptr(), kv_lens.data_ptr(), n_pages, page, heads, dim, max_pages, n_seqs, n_tokens, 0), dev, n_seqs, heads, dim
 
 
-def _heads(op: str, name: str, t, tokens: int, heads: int | None, dim: int, dtype=None):
+def _heads(op: str, name: str, t, tokens: int, heads: int, dim: int, dev: int, dtype):
     """Checks a [tokens, heads, dim] tensor and returns its (token, head) strides."""
-    if t.dim() != 3 or t.shape[0] != tokens or t.shape[2] != dim or (heads is not None and t.shape[1] != heads):
-        _refuse(_lib.ERR_SHAPE, f"{op}: {name} is {tuple(t.shape)}, not [{tokens}, {heads or 'heads'}, {dim}]")
-    if not t.is_cuda or (dtype is not None and t.dtype != dtype):
-        _refuse(_lib.ERR_ARGS, f"{op}: {name} must be a device tensor" + (f" of {dtype}" if dtype is not None else ""))
+    if t.shape != (tokens, heads, dim):
+        _refuse(_lib.ERR_SHAPE, f"{op}: {name} is {tuple(t.shape)}, not [{tokens}, {heads}, {dim}]")
+    if t.get_device() != dev or (dtype is not None and t.dtype != dtype):
+        _refuse(_lib.ERR_ARGS, f"{op}: {name} must be a tensor on the caches' device" + (f" of {dtype}" if dtype is not None else ""))
     a, b, c = t.stride()
     if c != 1:
         _refuse(_lib.ERR_ARGS, f"{op}: the last dimension of {name} must be dense")
     return a, b
+
+
+def _vector(op: str, name: str, t, n: int, dtype, dev: int) -> int:
+    """The address of an optional vector, 0 for None."""
+    if t is None:
+        return 0
+    if t.dtype != dtype or t.numel() != n or not t.is_contiguous() or t.get_device() != dev:
+        _refuse(_lib.ERR_ARGS, f"{op}: {name} must be {n} contiguous {dtype} on the caches' device")
+    return t.data_ptr()
 
 
 def rope_frequencies(rotary_dim: int, base: float = 10000.0, *, scaling: str = "none", factor: float = 1.0,
@@ -113,26 +155,24 @@ def rope_append(q, k, v, k_cache, v_cache, page_table, q_start, kv_lens, turns, 
     if q.dim() != 3:
         _refuse(_lib.ERR_SHAPE, f"rope_append: q is {tuple(q.shape)}, not [tokens, heads, dim]")
     T, hq, _ = q.shape
-    kv = _paged("rope_append", T, k_cache, v_cache, page_table, q_start, kv_lens)
+    kv, dev, _, hk, dim = _paged("rope_append", T, k_cache, v_cache, page_table, q_start, kv_lens)
     if layout not in _LAYOUTS:
         _refuse(_lib.ERR_ARGS, f"rope_append: unknown layout {layout!r} (half, interleaved)")
-    if turns.dtype != torch.float64 or turns.dim() != 1 or not turns.is_contiguous() or not turns.is_cuda:
-        _refuse(_lib.ERR_ARGS, "rope_append: turns must be a contiguous float64 device vector")
-    if positions is not None and (positions.dtype != torch.int32 or positions.numel() != T or
-                                  not positions.is_contiguous() or not positions.is_cuda):
-        _refuse(_lib.ERR_ARGS, "rope_append: positions must be int32 [tokens] on the device")
-    if k.dtype != q.dtype or v.dtype != q.dtype:
-        _refuse(_lib.ERR_ARGS, "rope_append: q, k and v must share one element type")
-    qs = _heads("rope_append", "q", q, T, hq, kv.head_dim)
-    ks = _heads("rope_append", "k", k, T, kv.kv_heads, kv.head_dim)
-    vs = _heads("rope_append", "v", v, T, kv.kv_heads, kv.head_dim)
+    dtype = q.dtype
+    qs = _heads("rope_append", "q", q, T, hq, dim, dev, None)
+    ks = _heads("rope_append", "k", k, T, hk, dim, dev, dtype)
+    vs = _heads("rope_append", "v", v, T, hk, dim, dev, dtype)
     if q_out is None:
-        q_out = torch.empty((T, hq, kv.head_dim), dtype=torch.bfloat16, device=q.device)
-    os_ = _heads("rope_append", "q_out", q_out, T, hq, kv.head_dim, torch.bfloat16)
-    args = _lib.Rope(q.data_ptr(), k.data_ptr(), v.data_ptr(), q_out.data_ptr(), *qs, *ks, *vs, *os_, turns.data_ptr(),
-                     None if positions is None else positions.data_ptr(), _dtype_code(q), hq, turns.numel(),
-                     _LAYOUTS[layout], magnitude, 0)
-    check(load().bybycu_rope_append(kv, args, _stream_ptr(stream)))
+        q_out = torch.empty((T, hq, dim), dtype=torch.bfloat16, device=q.device)
+        os_ = hq * dim, dim
+    else:
+        os_ = _heads("rope_append", "q_out", q_out, T, hq, dim, dev, torch.bfloat16)
+    pairs = turns.numel()
+    args = _ROPE(q.data_ptr(), k.data_ptr(), v.data_ptr(), q_out.data_ptr(), *qs, *ks, *vs, *os_,
+                 _vector("rope_append", "turns", turns, pairs, torch.float64, dev),
+                 _vector("rope_append", "positions", positions, T, torch.int32, dev), _dtype_code(q), hq, pairs,
+                 _LAYOUTS[layout], magnitude, 0)
+    check(_call("bybycu_rope_append")(kv, args, _stream("rope_append", dev, stream)))
     return q_out
 
 
@@ -151,22 +191,17 @@ def paged_attention(q, k_cache, v_cache, page_table, q_start, kv_lens, *, max_q:
     if q.dim() != 3:
         _refuse(_lib.ERR_SHAPE, f"paged_attention: q is {tuple(q.shape)}, not [tokens, heads, dim]")
     T, hq, _ = q.shape
-    kv = _paged("paged_attention", T, k_cache, v_cache, page_table, q_start, kv_lens)
-    qs = _heads("paged_attention", "q", q, T, hq, kv.head_dim, torch.bfloat16)
+    kv, dev, n_seqs, _, dim = _paged("paged_attention", T, k_cache, v_cache, page_table, q_start, kv_lens)
+    qs = _heads("paged_attention", "q", q, T, hq, dim, dev, torch.bfloat16)
     if out is None:
-        out = torch.empty((T, hq, kv.head_dim), dtype=torch.bfloat16 if out_dtype is None else out_dtype, device=q.device)
-    elif out_dtype is not None and out.dtype != out_dtype:
-        _refuse(_lib.ERR_ARGS, f"paged_attention: out is {out.dtype}, out_dtype {out_dtype}")
-    os_ = _heads("paged_attention", "out", out, T, hq, kv.head_dim)
-    if slopes is not None and (slopes.dtype != torch.float32 or slopes.numel() != hq or not slopes.is_contiguous() or not slopes.is_cuda):
-        _refuse(_lib.ERR_ARGS, "paged_attention: slopes must be float32 [heads] on the device")
-    if prefix_lens is not None and (prefix_lens.dtype != torch.int32 or prefix_lens.numel() != kv.n_seqs or
-                                    not prefix_lens.is_contiguous() or not prefix_lens.is_cuda):
-        _refuse(_lib.ERR_ARGS, "paged_attention: prefix_lens must be int32 [sequences] on the device")
-    args = _lib.Attention(q.data_ptr(), out.data_ptr(), *qs, *os_, None if slopes is None else slopes.data_ptr(),
-                          None if prefix_lens is None else prefix_lens.data_ptr(), _dtype_code(out), hq, max_q, max_kv,
-                          window, route, kv.head_dim ** -0.5 if scale is None else scale, softcap)
-    check(load().bybycu_paged_attention(kv, args, _stream_ptr(stream)))
+        out = torch.empty((T, hq, dim), dtype=torch.bfloat16 if out_dtype is None else out_dtype, device=q.device)
+        os_ = hq * dim, dim
+    else:
+        os_ = _heads("paged_attention", "out", out, T, hq, dim, dev, out_dtype)
+    args = _ATTENTION(q.data_ptr(), out.data_ptr(), *qs, *os_, _vector("paged_attention", "slopes", slopes, hq, torch.float32, dev),
+                      _vector("paged_attention", "prefix_lens", prefix_lens, n_seqs, torch.int32, dev), _dtype_code(out), hq,
+                      max_q, max_kv, window, route, dim ** -0.5 if scale is None else scale, softcap)
+    check(_call("bybycu_paged_attention")(kv, args, _stream("paged_attention", dev, stream)))
     return out
 
 
@@ -175,29 +210,33 @@ def copy_pages(k_cache, v_cache, pairs, *, stream=None) -> None:
     array, or a list), in every layer of caches [layers, pages, ...] (bf16 or any other type; 4-D
     [pages, ...] for one layer), in one launch.  The pairs act at once: no destination may be in
     another pair."""
-    import numpy as np
+    import torch
     if v_cache is not None and (v_cache.shape != k_cache.shape or v_cache.stride() != k_cache.stride() or v_cache.dtype != k_cache.dtype):
         _refuse(_lib.ERR_ARGS, "copy_pages: the caches must share shape, strides and type")
-    if k_cache.dim() not in (4, 5):
-        _refuse(_lib.ERR_SHAPE, f"copy_pages: caches are {tuple(k_cache.shape)}, not [layers, pages, heads, page size, dim]")
-    if not k_cache.is_cuda or (v_cache is not None and not v_cache.is_cuda):
+    shape, strides = k_cache.shape, k_cache.stride()
+    if len(shape) not in (4, 5):
+        _refuse(_lib.ERR_SHAPE, f"copy_pages: caches are {tuple(shape)}, not [layers, pages, heads, page size, dim]")
+    dev = k_cache.get_device()
+    if dev < 0 or (v_cache is not None and v_cache.get_device() != dev):
         _refuse(_lib.ERR_ARGS, "copy_pages: the caches must be on the device")
-    layers, layer_stride = (k_cache.shape[0], k_cache.stride(0)) if k_cache.dim() == 5 else (1, 0)
-    n_pages, page_stride = k_cache.shape[-4], k_cache.stride(-4)
-    inner = sorted((st, n) for st, n in zip(k_cache.stride()[-3:], k_cache.shape[-3:]) if n > 1)
-    dense = 1
-    for st, n in inner:
-        if st != dense:
-            _refuse(_lib.ERR_ARGS, "copy_pages: a page must be one dense block")
-        dense *= n
+    layers, layer_stride = (shape[0], strides[0]) if len(shape) == 5 else (1, 0)
+    n_pages, page_stride = shape[-4], strides[-4]
+    dense = shape[-3] * shape[-2] * shape[-1]
+    if not k_cache.is_contiguous():
+        run = 1
+        for st, n in sorted((st, n) for st, n in zip(strides[-3:], shape[-3:]) if n > 1):
+            if st != run:
+                _refuse(_lib.ERR_ARGS, "copy_pages: a page must be one dense block")
+            run *= n
     if n_pages == 1:
         page_stride = dense
-    p = np.ascontiguousarray(pairs, np.int32)
-    if p.size and (p.ndim != 2 or p.shape[1] != 2):
-        _refuse(_lib.ERR_SHAPE, f"copy_pages: pairs are {p.shape}, not [n, 2]")
+    p = torch.as_tensor(pairs, dtype=torch.int32, device="cpu").contiguous()
+    n = p.shape[0] if p.numel() else 0
+    if n and (p.dim() != 2 or p.shape[1] != 2):
+        _refuse(_lib.ERR_SHAPE, f"copy_pages: pairs are {tuple(p.shape)}, not [n, 2]")
     esz = k_cache.element_size()
-    check(load().bybycu_copy_pages(_ptr(k_cache), _ptr(v_cache), layers, layer_stride * esz, page_stride * esz, dense * esz,
-                                   n_pages, p.ctypes.data, p.shape[0] if p.size else 0, _stream_ptr(stream)))
+    check(_call("bybycu_copy_pages")(k_cache.data_ptr(), 0 if v_cache is None else v_cache.data_ptr(), layers, layer_stride * esz,
+                                     page_stride * esz, dense * esz, n_pages, p.data_ptr(), n, _stream("copy_pages", dev, stream)))
 
 
 def beam_select(logits, scores, keep: int, *, stream=None):
@@ -207,18 +246,20 @@ def beam_select(logits, scores, keep: int, *, stream=None):
     import torch
     if logits.dim() != 2 or scores.dim() != 2 or logits.shape[0] != scores.numel():
         _refuse(_lib.ERR_SHAPE, f"beam_select: logits {tuple(logits.shape)} for scores {tuple(scores.shape)}")
-    if scores.dtype != torch.float32 or not scores.is_contiguous() or not scores.is_cuda or not logits.is_cuda or \
-            (logits.shape[1] > 1 and logits.stride(1) != 1):
+    rows, vocab = logits.shape
+    stride, one = logits.stride()
+    dev = logits.get_device()
+    if scores.dtype != torch.float32 or not scores.is_contiguous() or dev < 0 or scores.get_device() != dev or (vocab > 1 and one != 1):
         _refuse(_lib.ERR_ARGS, "beam_select: scores must be contiguous float32, the rows of logits dense, both on the device")
     groups, beams = scores.shape
-    vocab = logits.shape[1]
     best = torch.empty((groups, keep), dtype=torch.float32, device=logits.device)
     which = torch.empty((2, groups, keep), dtype=torch.int32, device=logits.device)
-    stride = logits.stride(0) if logits.shape[0] > 1 else max(1, vocab)
-    check(load().bybycu_beam_select(_ptr(logits), _dtype_code(logits), stride, _ptr(scores), groups, beams, vocab, keep,
-                                    _ptr(best), C.c_void_p(which.data_ptr()), C.c_void_p(which.data_ptr() + 4 * groups * keep),
-                                    _stream_ptr(stream)))
-    return best, which[0], which[1]
+    at = which.data_ptr()
+    check(_call("bybycu_beam_select")(logits.data_ptr(), _dtype_code(logits), stride if rows > 1 else max(1, vocab), scores.data_ptr(),
+                                      groups, beams, vocab, keep, best.data_ptr(), at, at + 4 * groups * keep,
+                                      _stream("beam_select", dev, stream)))
+    beam, token = which.unbind(0)
+    return best, beam, token
 
 
 class PagedKvCache:
