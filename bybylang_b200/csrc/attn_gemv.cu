@@ -14,9 +14,10 @@
 //     probabilities stay in registers: the accumulator layout of S is the A layout of P.
 //   * fp32 output: P enters as three bf16 terms (24 bits), so the product with V is exact to fp32
 //     rounding; bf16 output: one rounding.
-//   * The cache axis is cut over the grid as well (splits of whole chunks); each split leaves
-//     unnormalised sums with their maximum, and a second, dependent launch joins them in a fixed
-//     order.
+//   * The cache axis is cut over the grid as well.  Up to 8 pieces are the CTAs of a cluster,
+//     which cuts each sequence's own keys evenly and joins its sums through distributed shared
+//     memory; more are splits of a fixed number of keys that leave unnormalised sums with their
+//     maximum for a second, dependent launch.  Both join in a fixed order.
 #include <algorithm>
 
 #include "attention.cuh"
@@ -53,6 +54,26 @@ __device__ __forceinline__ TileRange tile_range(const Params& p, const Seq& s, i
     r.lo_aligned = r.lo / align * align;
     r.splits = r.hi > r.lo_aligned ? 1 + (r.hi - r.lo_aligned - 1) / split_keys : 1;
     return r;
+}
+
+__device__ __forceinline__ void cluster_barrier() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Reads of the same shared-memory place in CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t cluster_addr(const void* p, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float2 cluster_load2(uint32_t addr) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 cluster_load4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
 }
 
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
@@ -95,8 +116,9 @@ struct GemvCfg {
     static constexpr int kLeast = 3 * kWK * kChunkBytes + kQBytes <= 227 * 1024 ? 3 : 2;
     static constexpr int kStages = kFit < kLeast ? kLeast : kFit > 8 ? 8 : kFit;
     static constexpr int kRingBytes = kWK * kStages * kChunkBytes;
-    // the end: every warp's sums [16][HD] fp32 and statistics, in the ring's place
-    static constexpr int kJoinBytes = kWarps * 16 * HD * 4;
+    // the end: every warp's sums [16][HD] fp32, and in a cluster the CTA's [16 WM][HD], in the ring's place
+    static constexpr int kCtaSums = kWarps * 16 * HD * 4;
+    static constexpr int kJoinBytes = kCtaSums + 16 * WM * HD * 4;
     static constexpr int kSmem = (kRingBytes > kJoinBytes ? kRingBytes : kJoinBytes) + kQBytes;
     static_assert(kSmem <= 227 * 1024, "shared memory");
 };
@@ -105,10 +127,11 @@ struct GemvCfg {
 // granules at a time and a batch ahead, so that no copy waits for the page table.
 template <int HD, int WM, bool F32, bool P16>
 __global__ void __launch_bounds__(128) attention_gemv_kernel(const kvc::Cache c, const Params p, const Partials part,
-                                                             int split_keys, int row_tiles) {
+                                                             int split_keys, int row_tiles, int cluster) {
     using C = GemvCfg<HD, WM>;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ float s_m[4][16], s_l[4][16];
+    __shared__ float2 s_ml[16 * WM];
     pdl_launch_dependents();
     pdl_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
@@ -116,10 +139,16 @@ __global__ void __launch_bounds__(128) attention_gemv_kernel(const kvc::Cache c,
     const int kvh = blockIdx.y / row_tiles, first_row = blockIdx.y % row_tiles * (16 * WM), b = blockIdx.z, split = blockIdx.x;
     const Seq s = load_seq(c, p, b);
     const int rows = min(16 * WM, s.rows * p.group - first_row);
-    if (rows <= 0) return;
-    const TileRange range = tile_range(p, s, first_row, rows, 16, split_keys);
-    if (split >= range.splits) return;
-    const int seg_lo = range.lo_aligned + split * split_keys;
+    if (rows <= 0) return;   // every CTA of a cluster has the same rows
+    TileRange range = tile_range(p, s, first_row, rows, 16, cluster ? INT32_MAX : split_keys);
+    if (cluster) {   // this tile's own keys, evenly, in whole rounds of the CTA's chunks
+        const int last = max(range.hi - range.lo_aligned, 1) - 1;
+        split_keys = (last / cluster / 64 + 1) * 64;
+        range.splits = last / split_keys + 1;
+    }
+    if (split >= range.splits && !cluster) return;
+    // a CTA of a cluster without keys has an empty segment
+    const int seg_lo = split < range.splits ? range.lo_aligned + split * split_keys : range.hi;
     const int seg_hi = seg_lo + min(range.hi - seg_lo, split_keys);
     const int D = c.head_dim;
 
@@ -411,6 +440,11 @@ if constexpr (F32) {
             acc.z = fmaf(f, v.z, acc.z);
             acc.w = fmaf(f, v.w, acc.w);
         }
+        if (cluster) {
+            *reinterpret_cast<float4*>(smem + C::kCtaSums + (r * HD + d) * 4) = acc;
+            if (d == 0) s_ml[r] = make_float2(mx, sum);
+            continue;
+        }
         const int64_t token = s.q0 + (first_row + r) / p.group, head = kvh * p.group + (first_row + r) % p.group;
         if (range.splits > 1) {
             const int64_t at = split * part.rows + token * p.q_heads + head;
@@ -420,6 +454,29 @@ if constexpr (F32) {
         }
         store_row4<F32>(p, token, head, d, acc, sum);
     }
+    if (!cluster) return;
+    cluster_barrier();
+    for (int i = split * 128 + threadIdx.x; i < rows * (HD / 4); i += cluster * 128) {
+        const int r = i / (HD / 4), d = i % (HD / 4) * 4;
+        if (d >= D) continue;
+        float mx = -INFINITY;
+        for (int k = 0; k < range.splits; ++k) mx = fmaxf(mx, cluster_load2(cluster_addr(&s_ml[r], k)).x);
+        const float base = mx == -INFINITY ? 0.0f : mx;
+        float sum = 0.0f;
+        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int k = 0; k < range.splits; ++k) {
+            const float2 ml = cluster_load2(cluster_addr(&s_ml[r], k));
+            const float4 v = cluster_load4(cluster_addr(smem + C::kCtaSums + (r * HD + d) * 4, k));
+            const float f = ex2(ml.x - base);
+            sum = fmaf(f, ml.y, sum);
+            acc.x = fmaf(f, v.x, acc.x);
+            acc.y = fmaf(f, v.y, acc.y);
+            acc.z = fmaf(f, v.z, acc.z);
+            acc.w = fmaf(f, v.w, acc.w);
+        }
+        store_row4<F32>(p, s.q0 + (first_row + r) / p.group, kvh * p.group + (first_row + r) % p.group, d, acc, sum);
+    }
+    cluster_barrier();   // no CTA leaves while another may read its sums
 }
 
 // Joins the splits: a block a row (token, head), each warp a quarter of the splits, then the four
@@ -547,21 +604,33 @@ static int launch_gemv_tile(const kvc::Cache& c, const Params& p, const DeviceIn
     const int64_t units = static_cast<int64_t>(row_tiles) * c.kv_heads * c.n_seqs;
     const int slots = info.sm_count * (C::kSmem <= 113 * 1024 ? 2 : 1);
     const int64_t span = longest_span(p, 16 * WM);
-    // One sequence: as many splits as fill the card once.  More: their lengths may differ up to
-    // the longest, so pieces of a sixth of a CTA's share of half of the most there can be, whatever
-    // the lengths, keep the tail short.  256 keys at least: below, a split's own sums weigh.
-    const int64_t share = c.n_seqs == 1 ? ceil_div(span * units, slots) : ceil_div(span * units, 12 * slots);
+    // One sequence: as many pieces as fill the card once.  More: their lengths may differ up to the
+    // longest, so pieces of a sixth of a CTA's share of half of the most there can be, whatever the
+    // lengths, keep the tail short.  128 keys at least (two rounds of a CTA's chunks).
+    const int64_t share = std::max<int64_t>(c.n_seqs == 1 ? ceil_div(span * units, slots) : ceil_div(span * units, 12 * slots), 128);
+    const int64_t pieces = ceil_div(span, share);
+    // A cluster where one wave holds them all: with more work than that its CTAs, which end
+    // together, keep SM slots from others (64 sequences of up to 8192: 216 us against 142).
+    const int fit = pieces == 1 || pieces > 12 ? 0 : pieces == 2 ? 2 : pieces <= 4 ? 4 : 8;
+    const int cluster = units * fit <= slots ? fit : 0;
+    // splits of the second kernel: 256 keys at least, below a split's own sums weigh
     const int split_keys = static_cast<int>(std::min<int64_t>(std::max<int64_t>(ceil_div(share, 64) * 64, 256), INT32_MAX / 2 / 64 * 64));
-    const int splits = static_cast<int>(ceil_div(span + 16, split_keys));
+    const int splits = cluster ? cluster : pieces == 1 ? 1 : static_cast<int>(ceil_div(span + 16, split_keys));
     Partials part{};
     SplitScratchMem scratch;
-    if (splits > 1)
+    if (splits > 1 && !cluster)
         if (int rc = scratch.take(info.device, static_cast<int64_t>(c.n_tokens) * p.q_heads, splits, c.head_dim, stream, &part)) return rc;
-    cudaLaunchAttribute attr[1];
-    const cudaLaunchConfig_t cfg = pdl_config(dim3(static_cast<unsigned>(splits), static_cast<unsigned>(row_tiles * c.kv_heads),
-                                                   static_cast<unsigned>(c.n_seqs)), 128, C::kSmem, stream, attr);
-    BYBYCU_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, c, p, part, split_keys, row_tiles));
-    return splits > 1 ? launch_join(c, p, part, split_keys, 16 * WM, 16, F32, stream) : BYBYCU_OK;
+    cudaLaunchAttribute attr[2];
+    cudaLaunchConfig_t cfg = pdl_config(dim3(static_cast<unsigned>(splits), static_cast<unsigned>(row_tiles * c.kv_heads),
+                                             static_cast<unsigned>(c.n_seqs)), 128, C::kSmem, stream, attr);
+    if (cluster) {
+        attr[1].id = cudaLaunchAttributeClusterDimension;
+        attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+        attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+        cfg.numAttrs = 2;
+    }
+    BYBYCU_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, c, p, part, splits == 1 ? INT32_MAX : split_keys, row_tiles, cluster));
+    return splits > 1 && !cluster ? launch_join(c, p, part, split_keys, 16 * WM, 16, F32, stream) : BYBYCU_OK;
 }
 
 template <int HD, bool F32>
