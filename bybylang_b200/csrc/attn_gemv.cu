@@ -166,7 +166,9 @@ __global__ void __launch_bounds__(128) attention_gemv_kernel(const kvc::Cache c,
             if (p.slopes) slope[i] = p.slopes[kvh * p.group + (first_row + r) % p.group] * kLog2e;
         }
     }
-    const bool mod = p.cap > 0.0f || p.slopes;
+    // the plain form takes the maximum of unscaled scores: a scale above 0 only
+    const bool mod = p.cap > 0.0f || p.slopes || !(p.scale_log2 > 0.0f);
+    const float unit = mod ? 1.0f : p.scale_log2;
     // keys that every row of the warp sees need no mask
     int all_lo = max(row_lo[0], row_lo[1]), all_hi = min(row_hi[0], row_hi[1]);
 #pragma unroll
@@ -232,10 +234,16 @@ __global__ void __launch_bounds__(128) attention_gemv_kernel(const kvc::Cache c,
         if (n_mine > 0) next_id = look_up(0);
     }
     int64_t granule = -1;   // this lane's granule: element offset of its first slot, -1 without one
+    // dense slots of the kernel's own head dimension: every copy's address is one base and a constant
+    const bool dense = P16 && D == HD && c.token_stride == HD;
+    const int64_t mine_off = head_off + row0 * c.token_stride + piece * 8;
+    const uint32_t mine_dst = my_ring + row0 * C::kPitch + piece * 16;
+    int fetch_stage = 0;
     auto fetch = [&](int i) {
         if (i < n_mine) {
             const int j0 = seg_lo + (wk + i * C::kWK) * C::kKC;
-            const uint32_t dst = my_ring + i % C::kStages * C::kChunkBytes + row0 * C::kPitch + piece * 16;
+            const uint32_t dst = mine_dst + fetch_stage * C::kChunkBytes;
+            fetch_stage = fetch_stage + 1 == C::kStages ? 0 : fetch_stage + 1;
             if constexpr (P16) {
                 if (i % kBatch == 0) {
                     batch_id = next_id;
@@ -252,6 +260,23 @@ __global__ void __launch_bounds__(128) attention_gemv_kernel(const kvc::Cache c,
 #pragma unroll
                 for (int w = 0; w < WM; ++w) at[w] = __shfl_sync(~0u, granule, i % kBatch * WM + w);
                 const bool whole = j0 >= range.lo && j0 + C::kKC <= seg_hi;
+                bool pages = true;
+#pragma unroll
+                for (int w = 0; w < WM; ++w) pages = pages && at[w] >= 0;
+                if (dense && whole && pages) {
+#pragma unroll
+                    for (int w = 0; w < WM; ++w) {
+                        const __nv_bfloat16 *kp = c.k + (at[w] + mine_off), *vp = c.v + (at[w] + mine_off);
+#pragma unroll
+                        for (int r = 0; r < 16 / kRowStep; ++r) {
+                            const uint32_t to = dst + (w * 16 + r * kRowStep) * C::kPitch;
+                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(kp + r * kRowStep * HD) : "memory");
+                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + C::kTensorBytes), "l"(vp + r * kRowStep * HD) : "memory");
+                        }
+                    }
+                    asm volatile("cp.async.commit_group;" ::: "memory");
+                    return;
+                }
 #pragma unroll
                 for (int r = 0; r < C::kKC / kRowStep; ++r) {
                     const int j = row0 + r * kRowStep;   // its granule is r * kRowStep / 16: kRowStep divides 16
@@ -294,12 +319,14 @@ __global__ void __launch_bounds__(128) attention_gemv_kernel(const kvc::Cache c,
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int i = 0; i < C::kStages - 1; ++i) fetch(i);
+    int stage = 0;
     for (int i = 0; i < n_mine; ++i) {
         asm volatile("cp.async.wait_group %0;" ::"n"(C::kStages - 2) : "memory");
         group_sync();   // the chunk is whole, and the slot that the next fetch fills is free
         fetch(i + C::kStages - 1);
         const int j0 = seg_lo + (wk + i * C::kWK) * C::kKC;
-        const uint32_t kc = my_ring + i % C::kStages * C::kChunkBytes, vc = kc + C::kTensorBytes;
+        const uint32_t kc = my_ring + stage * C::kChunkBytes, vc = kc + C::kTensorBytes;
+        stage = stage + 1 == C::kStages ? 0 : stage + 1;
         float sc[C::kKC / 8][4] = {};
 #pragma unroll
         for (int k = 0; k < kSteps; ++k) {
@@ -315,16 +342,23 @@ __global__ void __launch_bounds__(128) attention_gemv_kernel(const kvc::Cache c,
             }
         }
         const bool masked = j0 < all_lo || j0 + C::kKC > all_hi;
+        if (mod) {
 #pragma unroll
-        for (int n = 0; n < C::kKC / 8; ++n)
+            for (int n = 0; n < C::kKC / 8; ++n)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int j = j0 + n * 8 + t4 * 2 + (e & 1), r = e >> 1;
-                if (mod) sc[n][e] = score_log2<true>(p, sc[n][e], slope[r], row_pos[r] - j);
-                else sc[n][e] *= p.scale_log2;
-                if (masked && (j < row_lo[r] || j >= row_hi[r])) sc[n][e] = -INFINITY;
-            }
-        float mn[2] = {m[0], m[1]};
+                for (int e = 0; e < 4; ++e)
+                    sc[n][e] = score_log2<true>(p, sc[n][e], slope[e >> 1], row_pos[e >> 1] - (j0 + n * 8 + t4 * 2 + (e & 1)));
+        }
+        if (masked) {
+#pragma unroll
+            for (int n = 0; n < C::kKC / 8; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int j = j0 + n * 8 + t4 * 2 + (e & 1);
+                    if (j < row_lo[e >> 1] || j >= row_hi[e >> 1]) sc[n][e] = -INFINITY;
+                }
+        }
+        float mn[2] = {-INFINITY, -INFINITY};
 #pragma unroll
         for (int n = 0; n < C::kKC / 8; ++n) {
             mn[0] = fmaxf(mn[0], fmaxf(sc[n][0], sc[n][1]));
@@ -334,14 +368,18 @@ __global__ void __launch_bounds__(128) attention_gemv_kernel(const kvc::Cache c,
         for (int r = 0; r < 2; ++r) {
             mn[r] = fmaxf(mn[r], __shfl_xor_sync(~0u, mn[r], 1));
             mn[r] = fmaxf(mn[r], __shfl_xor_sync(~0u, mn[r], 2));
+            mn[r] = fmaxf(m[r], mn[r] * unit);
         }
-        float base[2], keep[2];
+        // The sums follow a new maximum only when one grew by more than 2^8 (probabilities are then
+        // below 2^8 with the same relative rounding): hardly ever after the first chunks.
+        if (__any_sync(~0u, mn[0] > m[0] + 8.0f || mn[1] > m[1] + 8.0f)) {
+            float keep[2];
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            base[r] = mn[r] == -INFINITY ? 0.0f : mn[r];
-            keep[r] = ex2(m[r] - base[r]);
-        }
-        if (__any_sync(~0u, mn[0] != m[0] || mn[1] != m[1])) {
+            for (int r = 0; r < 2; ++r) {
+                keep[r] = mn[r] == -INFINITY ? 1.0f : ex2(m[r] - mn[r]);
+                l[r] *= keep[r];
+                m[r] = mn[r];
+            }
 #pragma unroll
             for (int n = 0; n < HD / 8; ++n) {
                 o[n][0] *= keep[0];
@@ -349,15 +387,12 @@ __global__ void __launch_bounds__(128) attention_gemv_kernel(const kvc::Cache c,
                 o[n][2] *= keep[1];
                 o[n][3] *= keep[1];
             }
-            l[0] *= keep[0];
-            l[1] *= keep[1];
-            m[0] = mn[0];
-            m[1] = mn[1];
         }
+        const float off[2] = {m[0] == -INFINITY ? 0.0f : -m[0], m[1] == -INFINITY ? 0.0f : -m[1]};
 #pragma unroll
         for (int n = 0; n < C::kKC / 8; ++n) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sc[n][e] = ex2(sc[n][e] - base[e >> 1]);
+            for (int e = 0; e < 4; ++e) sc[n][e] = ex2(fmaf(sc[n][e], unit, off[e >> 1]));
             l[0] += sc[n][0] + sc[n][1];
             l[1] += sc[n][2] + sc[n][3];
         }
