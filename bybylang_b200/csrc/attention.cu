@@ -143,8 +143,11 @@ extern "C" int bybycu_paged_attention(const bybycu_paged_kv* kv, const bybycu_at
     if (a->route == BYBYCU_ROUTE_TC && !tc)
         return set_error(BYBYCU_ERR_SHAPE, "paged_attention: the tensor-core route needs bf16 output, head dimension <= 128, at most "
                                            "128 heads a group and pages of 8, 16, 32, 64 or a multiple of 128 tokens");
-    // one tensor-core tile is 128 rows
-    if (a->route == BYBYCU_ROUTE_TC || (a->route == BYBYCU_ROUTE_AUTO && tc && static_cast<int64_t>(a->max_q) * p.group > 64))
+    // A tensor-core tile costs its 128 rows however many there are, the GEMV's warps 16 each: 8
+    // sequences of 4096 keys, 8 kv heads of 128, at 16, 32, 64 and 128 rows 51, 64, 88, 153 us on
+    // the GEMV and 43, 46, 51, 61 on the tensor cores; heads of 64 33, 41, 53, 93 and 37, 39, 43,
+    // 53; one sequence of 2048 15, 17, 21, 23 and 19, 19, 20, 23.
+    if (a->route == BYBYCU_ROUTE_TC || (a->route == BYBYCU_ROUTE_AUTO && tc && static_cast<int64_t>(a->max_q) * p.group > 32))
         return attn::launch_tc_attention(c, p, mod, s);
     return attn::launch_gemv(c, p, f32, s);
 }

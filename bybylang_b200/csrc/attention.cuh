@@ -53,12 +53,24 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+// The smaller and the larger of two numbers, NaN where either is: a NaN score is not clamped away.
+__device__ __forceinline__ float min_nan(float a, float b) {
+    float d;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+
 // cap * tanh(y) of two scores in units of log2, y = raw * scale / cap: tanh(y) = 1 - 2 / (1 + e^2y)
 // with the hardware's exponential and one reciprocal for both.  The absolute error is a few
 // 2^-24 times the cap.  2 y log2(e) is held below 60, where tanh is 1 in fp32, so that the
 // product of the two denominators stays finite.
 __device__ __forceinline__ float2 capped_log2(const Params& p, float raw0, float raw1) {
-    const float a = 1.0f + ex2(fminf(raw0 * p.cap_in, 60.0f)), b = 1.0f + ex2(fminf(raw1 * p.cap_in, 60.0f));
+    const float a = 1.0f + ex2(min_nan(raw0 * p.cap_in, 60.0f)), b = 1.0f + ex2(min_nan(raw1 * p.cap_in, 60.0f));
     float r;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(a * b));
     return make_float2(fmaf(-2.0f * p.cap_out, r * b, p.cap_out), fmaf(-2.0f * p.cap_out, r * a, p.cap_out));

@@ -514,9 +514,10 @@ if constexpr (F32) {
     cluster_barrier();   // no CTA leaves while another may read its sums
 }
 
-// Joins the splits: a block a row (token, head), each warp a quarter of the splits, then the four
-// in order.
-template <bool F32>
+// Joins the splits of a row (token, head): WARPS warps of a block take equal runs of them, and are
+// added in order.  Four warps for many splits and few rows (a warp alone took 22 us for 37), one a
+// row for many rows.
+template <bool F32, int WARPS>
 __global__ void __launch_bounds__(128) attention_join_kernel(const kvc::Cache c, const Params p, const Partials part,
                                                              int split_keys, int tile_rows, int align) {
     __shared__ float s_sum[4];
@@ -524,7 +525,8 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const kvc::Cache c,
     pdl_launch_dependents();
     pdl_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t row = blockIdx.x;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * (4 / WARPS) + warp / WARPS;
+    if (row >= part.rows) return;
     const int t = static_cast<int>(row / p.q_heads), h = static_cast<int>(row % p.q_heads), D = c.head_dim;
     int b = 0;
     for (int i = 0; i < c.n_seqs; i += 32) b += __popc(__ballot_sync(~0u, i + lane < c.n_seqs && c.q_start[i + lane + 1] <= t));
@@ -540,7 +542,7 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const kvc::Cache c,
 #pragma unroll
     for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, o));
     const float base = mx == -INFINITY ? 0.0f : mx;
-    const int per = (range.splits + 3) / 4, k0 = warp * per, k1 = min(range.splits, k0 + per);
+    const int per = (range.splits + WARPS - 1) / WARPS, k0 = warp % WARPS * per, k1 = min(range.splits, k0 + per);
     for (int d0 = 0; d0 < D; d0 += 128) {
         const int d = d0 + lane * 4;
         float sum = 0.0f;
@@ -557,18 +559,22 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const kvc::Cache c,
                 acc.z = fmaf(f, v.z, acc.z);
                 acc.w = fmaf(f, v.w, acc.w);
             }
-            if (warp) s_acc[warp - 1][d / 4] = acc;
         }
-        if (lane == 0) s_sum[warp] = sum;
-        __syncthreads();
-        if (warp == 0 && d < D) {
-            for (int w = 0; w < 3; ++w) {
-                const float4 v = s_acc[w][d / 4];
-                acc = make_float4(acc.x + v.x, acc.y + v.y, acc.z + v.z, acc.w + v.w);
+        if constexpr (WARPS == 4) {   // the whole block has one row
+            if (warp && d < D) s_acc[warp - 1][d / 4] = acc;
+            if (lane == 0) s_sum[warp] = sum;
+            __syncthreads();
+            if (warp == 0 && d < D) {
+                for (int w = 0; w < 3; ++w) {
+                    const float4 v = s_acc[w][d / 4];
+                    acc = make_float4(acc.x + v.x, acc.y + v.y, acc.z + v.z, acc.w + v.w);
+                }
+                store_row4<F32>(p, t, h, d, acc, s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3]);
             }
-            store_row4<F32>(p, t, h, d, acc, s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3]);
+            __syncthreads();
+        } else if (d < D) {
+            store_row4<F32>(p, t, h, d, acc, sum);
         }
-        __syncthreads();
     }
 }
 
@@ -588,10 +594,12 @@ static cudaLaunchConfig_t pdl_config(dim3 grid, int threads, size_t smem, cudaSt
 
 static int launch_join(const kvc::Cache& c, const Params& p, const Partials& part, int split_keys, int tile_rows,
                        int align, bool f32, cudaStream_t stream) {
+    const bool wide = part.rows <= 4096;
     cudaLaunchAttribute attr[1];
-    const cudaLaunchConfig_t cfg = pdl_config(dim3(static_cast<unsigned>(part.rows)), 128, 0, stream, attr);
-    BYBYCU_CUDA_TRY(cudaLaunchKernelEx(&cfg, f32 ? attention_join_kernel<true> : attention_join_kernel<false>, c, p, part,
-                                       split_keys, tile_rows, align));
+    const cudaLaunchConfig_t cfg = pdl_config(dim3(static_cast<unsigned>(wide ? part.rows : ceil_div(part.rows, 4))), 128, 0, stream, attr);
+    auto kern = wide ? (f32 ? attention_join_kernel<true, 4> : attention_join_kernel<false, 4>)
+                     : (f32 ? attention_join_kernel<true, 1> : attention_join_kernel<false, 1>);
+    BYBYCU_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, c, p, part, split_keys, tile_rows, align));
     return BYBYCU_OK;
 }
 
@@ -637,7 +645,7 @@ static int launch_gemv_tile(const kvc::Cache& c, const Params& p, const DeviceIn
     if (static_cast<int64_t>(row_tiles) * c.kv_heads > 65535 || c.n_seqs > 65535)
         return set_error(BYBYCU_ERR_SHAPE, "paged_attention: %d sequences, %d kv heads, %d new tokens", c.n_seqs, c.kv_heads, p.max_q);
     const int64_t units = static_cast<int64_t>(row_tiles) * c.kv_heads * c.n_seqs;
-    const int slots = info.sm_count * (C::kSmem <= 113 * 1024 ? 2 : 1);
+    const int slots = info.sm_count * std::max(1, std::min(3, static_cast<int>(227 * 1024 / (C::kSmem + 2048))));
     const int64_t span = longest_span(p, 16 * WM);
     // One sequence: as many pieces as fill the card once.  More: their lengths may differ up to the
     // longest, so pieces of a sixth of a CTA's share of half of the most there can be, whatever the

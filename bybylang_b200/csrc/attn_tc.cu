@@ -137,12 +137,6 @@ __device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, vo
     }
 }
 
-__device__ __forceinline__ float max_nan(float a, float b) {   // NaN where either is
-    float d;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-    return d;
-}
-
 // Whether any thread of a pair of warps says so; their barrier.
 __device__ __forceinline__ bool pair_any(uint32_t id, bool mine) {
     uint32_t any;
@@ -409,13 +403,12 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
         const int my_rows = min(tile_rows, rows - i * tile_rows);
         const int row = first_row + i * tile_rows + r;
         const bool real = r < my_rows;
-        const int pos = s.first_pos + row / p.group;
-        int row_lo = 0, row_hi = 0;
-        float slope = 0.0f;
-        if (real) {
-            row_range(p, s, pos, &row_lo, &row_hi);
-            if (MOD && p.slopes) slope = p.slopes[kvh * p.group + row % p.group] * kLog2e;
-        }
+        // a thread without a row looks where the tile's last row does, so that it needs no mask there
+        const int like = first_row + i * tile_rows + max(0, min(r, my_rows - 1));
+        const int pos = s.first_pos + like / p.group;
+        int row_lo, row_hi;
+        row_range(p, s, pos, &row_lo, &row_hi);
+        const float slope = MOD && p.slopes ? p.slopes[kvh * p.group + like % p.group] * kLog2e : 0.0f;
         // f(this thread's value, its row's other value), the same in both: by the second half's thread
         float* place = reinterpret_cast<float*>(smem + C::kOffRow) + i * kRows + r;
         auto join = [&](float mine, auto f) {
@@ -435,12 +428,22 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
             __syncwarp();
             tc::tc_fence_after();
             const int t0 = seg_lo + j * kKeys + half * kHalf;
-            // 32 of this thread's scores, in the units of the sum to come, -inf where the row may not look
+            // 32 of this thread's scores as the tensor core left them
             auto load = [&](int q, uint32_t (&sc)[32]) {
                 tc::tmem_ld32(ts + 32 * q, sc);
                 tc::tc_wait_ld();
-                if constexpr (MOD) {
+            };
+            // in the units of the sum to come (MOD), -inf where the row may not look; whether that is anywhere
+            auto score = [&](int q, uint32_t (&sc)[32], bool mod) {
+                const int lo = row_lo - t0 - 32 * q, hi = row_hi - t0 - 32 * q;
+                const bool masked = __any_sync(~0u, lo > 0 || hi < 32);
+                if (mod) {
                     if (p.cap > 0.0f) {
+                        if (masked) {   // two scores share a reciprocal: nothing may come of a slot past the cache
+#pragma unroll
+                            for (int e = 0; e < 32; ++e)
+                                if (e < lo || e >= hi) sc[e] = 0u;
+                        }
 #pragma unroll
                         for (int e = 0; e < 32; e += 2) {
                             const float2 t = capped_log2(p, __uint_as_float(sc[e]), __uint_as_float(sc[e + 1]));
@@ -458,8 +461,6 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
                             sc[e] = __float_as_uint(fmaf(-slope, fabsf(dist - static_cast<float>(e)), __uint_as_float(sc[e])));
                     }
                 }
-                const int lo = row_lo - t0 - 32 * q, hi = row_hi - t0 - 32 * q;
-                const bool masked = __any_sync(~0u, lo > 0 || hi < 32);
                 if (masked) {
 #pragma unroll
                     for (int e = 0; e < 32; ++e)
@@ -477,14 +478,22 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
                 }
                 return max_nan(max3(mx[0], mx[1], mx[2]), mx[3]);
             };
-            // The first 32 scores stay in registers, the second come again after the maximum is
-            // known (registers left free let the exponentials overlap), unless they took work.
+            // The second 32 scores come again after the maximum is known (registers left free let the
+            // exponentials overlap); scores that took work go back to tensor memory for that.
             uint32_t first[32], second[32];
-            const bool masked0 = load(0, first);
-            bool masked1 = load(1, second);
-            float mn = max_nan(m, unit * max_nan(top(first), top(second)));   // a NaN score makes the row NaN
+            load(0, first);
+            const bool masked0 = score(0, first, MOD);
+            float mn = top(first);
+            if constexpr (MOD) tc::tmem_st32(ts, first);
+            load(1, second);
+            const bool masked1 = score(1, second, MOD);
+            mn = max_nan(m, unit * max_nan(mn, top(second)));   // a NaN score makes the row NaN
+            if constexpr (MOD) {
+                tc::tmem_st32(ts + 32, second);
+                tc::tc_wait_st();
+            }
             // Whether a row of this pair of warps (the two halves of 32 rows) needs a new maximum
-            if (pair_any(1 + i * 4 + (warp & 3), !(mn <= m + 8.0f) && mn != -INFINITY)) {
+            if (pair_any(1 + i * 4 + (warp & 3), real && !(mn <= m + 8.0f) && mn != -INFINITY)) {
                 mn = join(mn, [](float a, float b) { return max_nan(a, b); });
                 const float f = mn == -INFINITY ? 1.0f : ex2(m - mn);
                 l *= f;
@@ -522,9 +531,11 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
                 }
                 tc::tmem_st16(ts + 16 * q, pk);
             };
+            if constexpr (MOD) load(0, first);
             if (masked0) probabilities(first, 0, std::false_type{});
             else probabilities(first, 0, std::true_type{});
-            if constexpr (!MOD) masked1 = load(1, second);
+            load(1, second);
+            if constexpr (!MOD) score(1, second, false);
             if (masked1) probabilities(second, 1, std::false_type{});
             else probabilities(second, 1, std::true_type{});
             tc::tc_wait_st();
