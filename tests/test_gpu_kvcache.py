@@ -400,3 +400,131 @@ def test_beam_select_hard_rows(what, vocab, dtype):
     elif what == "blocks":     # whole warps' tokens masked, the rest all above them
         x = torch.where((torch.arange(vocab) // 128) % 8 == 3, -math.inf, x + 10)
     check_beams(x.to(dtype).to(DEV), s.to(DEV), keep)
+
+
+# ---- together, and at the edges of the address space ----------------------------------------
+
+def test_beam_search_example():
+    """The example's found sequences, scored again without a cache in fp32: q, k, v, the attention
+    output and the activations of the 4-bit products are rounded to 8..15 bits on the way, which at
+    these widths moves a log-probability by some 1e-2; a wrong page, position or parent by whole
+    units."""
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "beam_search.py")
+    spec = importlib.util.spec_from_file_location("beam_search_example", path)
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    model, prompts, found = mod.main(["--beams", "3", "--tokens", "20", "--prompts", "2"])
+    assert _lib.device_error() == 0
+    assert model.pool.free_pages == model.pool.n_pages          # every page came back
+    for prompt, beams in zip(prompts, found):
+        assert [s for s, _ in beams] == sorted((s for s, _ in beams), reverse=True)
+        assert len({tuple(t) for _, t in beams}) == len(beams)
+        for score, text in beams:
+            assert abs(score - model.check(prompt, text)) < 0.2
+
+
+def test_offsets_past_32_bits():
+    """Pages that start 2^31 elements and more into the cache."""
+    page, heads, dim = 64, 8, 128
+    per = page * heads * dim
+    n = (1 << 31) // per + 40
+    k = torch.empty(n, heads, page, dim, dtype=torch.bfloat16, device=DEV)
+    v = torch.empty(n, heads, page, dim, dtype=torch.bfloat16, device=DEV)
+    lens = [(1, 200), (70, 100)]
+    bt = Batch(lens, page=page, heads=16, kv_heads=heads, dim=dim, seed=3)
+    for i in range(bt.n_pages):     # the same cache, far out
+        k[n - 1 - i], v[n - 1 - i] = bt.k[i], bt.v[i]
+    bt.table = torch.where(bt.table >= 0, n - 1 - bt.table, bt.table)
+    bt.k, bt.v = k, v
+    for route in (GEMV, TC, SIMT):
+        check(bt, route, torch.bfloat16)
+    x = torch.randn(71, 32, dim, device=DEV)
+    q, kk, vv = x.split([16, 8, 8], 1)
+    kv.rope_append(q, kk, vv, *bt.args(), kv.rope_frequencies(0, device=DEV))     # no pair turns: a plain append
+    torch.cuda.synchronize()
+    assert _lib.device_error() == 0
+    assert torch.equal(k[bt.table[0, 3].long(), :, 199 % page], kk[0].to(torch.bfloat16))
+    assert torch.equal(v[bt.table[1, 1].long(), :, 99 % page], vv[70].to(torch.bfloat16))
+    pairs = [(n - 1, 0), (1, n - 20)]
+    k[1].fill_(3.0)
+    kv.copy_pages(k, v, pairs)
+    torch.cuda.synchronize()
+    assert torch.equal(k[0].view(torch.int16), k[n - 1].view(torch.int16)) and (k[n - 20] == 3.0).all()
+
+
+@pytest.mark.parametrize("route", [GEMV, TC, SIMT])
+def test_attention_groups_and_rows_that_do_not_divide(route):
+    for heads, kv_heads, dim in ((100, 1, 64), (9, 3, 128), (127, 1, 32)):
+        bt = Batch([(3, 40), (20, 333), (1, 5)], page=16, heads=heads, kv_heads=kv_heads, dim=dim, seed=heads)
+        check(bt, route, torch.bfloat16)
+    bt = Batch([(3, 40), (2, 200)], page=16, heads=200, kv_heads=1, dim=64, seed=1)
+    if route == TC:
+        with pytest.raises(_lib.BybyCudaError, match="128 heads a group"):
+            kv.paged_attention(bt.q, *bt.args(), max_q=3, max_kv=200, route=TC)
+    else:
+        check(bt, route, torch.bfloat16)
+
+
+@pytest.mark.parametrize("route", [GEMV, TC, SIMT])
+def test_attention_nan_reaches_only_rows_that_see_it(route):
+    """A NaN key is a NaN row for every row that sees it, in whatever half or step of a block, and
+    nothing for the others; so is one behind a tanh cap."""
+    for softcap in (0.0, 20.0):
+        for at in (3, 37, 70, 127, 128, 199):
+            bt = Batch([(200, 200), (60, 200)], page=16, heads=2, kv_heads=1, dim=64, seed=at)
+            bt.k[bt.table[0, at // 16], 0, at % 16, 5] = float("nan")
+            out = kv.paged_attention(bt.q, *bt.args(), max_q=200, max_kv=200, softcap=softcap, out_dtype=torch.bfloat16, route=route)
+            torch.cuda.synchronize()
+            bad = torch.isnan(out).any(-1).any(-1)
+            want = torch.zeros(260, dtype=torch.bool, device=DEV)
+            want[at:200] = True
+            assert torch.equal(bad, want)
+    assert _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("route", [GEMV, TC, SIMT])
+def test_attention_is_the_same_every_time(route):
+    for lens in ([(1, 9000)], [(1, 700)] * 3, [(300, 2000), (64, 64)]):
+        bt = Batch(lens, page=64, heads=8, kv_heads=2, dim=128, seed=2)
+        outs = [kv.paged_attention(bt.q, *bt.args(), max_q=bt.max_q, max_kv=bt.max_kv, route=route) for _ in range(3)]
+        assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+
+
+def test_python_refusals():
+    bt = Batch([(1, 20)], page=16, heads=4, kv_heads=2, dim=64, seed=1)
+    call = dict(max_q=1, max_kv=20)
+    with pytest.raises(_lib.BybyCudaError, match="torch.bfloat16"):
+        kv.paged_attention(bt.q.float(), *bt.args(), **call)
+    with pytest.raises(_lib.BybyCudaError, match="torch.float32"):
+        kv.paged_attention(bt.q, *bt.args(), slopes=torch.zeros(3, device=DEV), **call)
+    with pytest.raises(_lib.BybyCudaError, match="torch.int32"):
+        kv.paged_attention(bt.q, *bt.args(), prefix_lens=torch.zeros(1, device=DEV), **call)
+    with pytest.raises(_lib.BybyCudaError, match="not \\[1, 4, 64\\]"):
+        kv.paged_attention(bt.q, *bt.args(), out=torch.zeros(2, 4, 64, dtype=torch.bfloat16, device=DEV), **call)
+    with pytest.raises(_lib.BybyCudaError, match="float32 or bfloat16"):
+        kv.paged_attention(bt.q, *bt.args(), out_dtype=torch.float16, **call)
+    with pytest.raises(_lib.BybyCudaError, match="16-byte aligned"):
+        odd = torch.zeros(4 * 64 + 1, dtype=torch.bfloat16, device=DEV)[1:].view(1, 4, 64)
+        kv.paged_attention(odd, *bt.args(), **call)
+    with pytest.raises(_lib.BybyCudaError, match="tensor-core route"):
+        kv.paged_attention(bt.q, *bt.args(), out_dtype=torch.float32, route=TC, **call)
+    q3 = torch.zeros(1, 3, 64, dtype=torch.bfloat16, device=DEV)
+    with pytest.raises(_lib.BybyCudaError, match="3 query heads over 2"):
+        kv.paged_attention(q3, *bt.args(), **call)
+    turns = kv.rope_frequencies(64, device=DEV)
+    kk = torch.zeros(1, 2, 64, device=DEV)
+    with pytest.raises(_lib.BybyCudaError, match="unknown layout"):
+        kv.rope_append(kk.expand(1, 2, 64), kk, kk, *bt.args(), turns, layout="other")
+    with pytest.raises(_lib.BybyCudaError, match="torch.float64"):
+        kv.rope_append(kk, kk, kk, *bt.args(), turns.float())
+    with pytest.raises(_lib.BybyCudaError, match="k must be"):
+        kv.rope_append(kk, kk.bfloat16(), kk, *bt.args(), turns)
+    with pytest.raises(_lib.BybyCudaError, match="dense block"):
+        kv.copy_pages(bt.k[:, :, :8], bt.v[:, :, :8], [(0, 1)])
+    with pytest.raises(_lib.BybyCudaError, match="scores must be contiguous"):
+        kv.beam_select(torch.zeros(2, 9, device=DEV), torch.zeros(1, 2, dtype=torch.float64, device=DEV), 2)
+    with pytest.raises(_lib.BybyCudaError, match="unknown scaling"):
+        kv.rope_frequencies(64, scaling="x", device=DEV)
+    assert _lib.device_error() == 0
