@@ -144,6 +144,39 @@ proc bybycu_upload_host_range*(dst, src: pointer; bytes: int64): cint
 proc bybycu_session_upload_ptr*(host: pointer; bytes: int64; handle: ptr pointer): cint
 proc bybycu_fingerprint*(data: pointer; bytes: int64; outp: cstring; outLen: cint): cint
 proc bybycu_checkpoint_index*(path: cstring; outp: ptr BybycuTensorInfo; cap: cint; count: ptr cint): cint
+# paged key/value cache and the operators around it (no reference counterpart: the structs are
+# those of bybycuda.h, field for field)
+type
+  BybycuPagedKv* {.importc: "bybycu_paged_kv", header: "bybycuda.h".} = object
+    k*, v*: pointer
+    page_stride*, head_stride*, token_stride*: int64
+    page_table*: ptr int32
+    table_stride*: int64
+    q_start*, kv_lens*: ptr int32
+    n_pages*, page_size*, kv_heads*, head_dim*, max_pages*, n_seqs*, n_tokens*, reserved*: int32
+  BybycuRope* {.importc: "bybycu_rope", header: "bybycuda.h".} = object
+    q*, k*, v*, q_out*: pointer
+    q_token_stride*, q_head_stride*, k_token_stride*, k_head_stride*, v_token_stride*, v_head_stride*: int64
+    out_token_stride*, out_head_stride*: int64
+    turns*: ptr float64
+    positions*: ptr int32
+    in_dtype*, q_heads*, pairs*, interleaved*: int32
+    magnitude*: float32
+    reserved*: int32
+  BybycuAttention* {.importc: "bybycu_attention", header: "bybycuda.h".} = object
+    q*, `out`*: pointer
+    q_token_stride*, q_head_stride*, out_token_stride*, out_head_stride*: int64
+    slopes*: ptr float32
+    prefix_lens*: ptr int32
+    out_dtype*, q_heads*, max_q*, max_kv*, window*, route*: int32
+    scale*, softcap*: float32
+proc bybycu_rope_append*(kv: ptr BybycuPagedKv; args: ptr BybycuRope; stream: pointer): cint
+proc bybycu_paged_attention*(kv: ptr BybycuPagedKv; args: ptr BybycuAttention; stream: pointer): cint
+proc bybycu_copy_pages*(k, v: pointer; nLayers: cint; layerStride, pageStride, pageBytes: int64;
+                       nPages: cint; pairs: ptr int32; nPairs: cint; stream: pointer): cint
+proc bybycu_beam_select*(logits: pointer; logitsDtype: cint; rowStride: int64; scores: ptr float32;
+                        groups, beams, vocab, keep: cint; outScores: ptr float32;
+                        outBeams, outTokens: ptr int32; stream: pointer): cint
 {.pop.}
 
 proc bybycuLastError*(): string =

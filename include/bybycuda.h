@@ -379,15 +379,18 @@ BYBYCU_API int bybycu_rope_append(const bybycu_paged_kv* kv, const bybycu_rope* 
  * over the positions j < kv_lens[b] with j <= p_i, or j < prefix_lens[b] where given, and, with
  * window > 0, p_i - j < window.  A row that sees no key gives zeros.  q head h reads kv head
  * h / (q_heads / kv_heads).  Cache slots past kv_lens[b] and pages that no new token sees are
- * not used, whatever they hold.
+ * not used, whatever they hold.  A key that a row does not see does not reach it; a value that is
+ * not finite does where another row of the same launch tile sees it (0 * NaN).
  *   max_q, max_kv bound the new tokens and the cache length of every sequence (the launch is sized
  *   by them); a sequence beyond either records device error 10 and its rows beyond are not
  *   computed.
- *   route AUTO: GEMV (warp-level MMAs, the cache split over the grid) for few query rows a kv
- *   head, TC (tcgen05) for more where the head dimension and page size allow, SIMT (one warp a
- *   row, fp32) for head dimensions that no other kernel is built for.
- * Scores, softmax statistics and sums are fp32; the probabilities enter the product with V as
- * bf16 for a bf16 output and as two bf16 terms (16 bits) for an fp32 output. */
+ *   route AUTO: TC (tcgen05) for more than 32 query rows (new tokens x heads of a group) a kv head
+ *   where it applies - bf16 output, head dimension up to 128, groups up to 128 heads, pages of 8,
+ *   16, 32, 64 or a multiple of 128 tokens - else GEMV (warp-level MMAs, the cache split over the
+ *   grid), which runs every shape.  SIMT: one warp a row, fp32 FMAs, every shape; only when asked
+ *   for.  An explicit TC that does not apply returns BYBYCU_ERR_SHAPE.
+ * Scores, softmax statistics and sums are fp32.  The probabilities enter the product with V as
+ * bf16 for a bf16 output, as three bf16 terms (24 bits) for an fp32 output (SIMT: fp32). */
 typedef struct bybycu_attention {
     const void* q;                  /* bf16 [n_tokens, q_heads, head_dim] */
     void* out;                      /* out_dtype, same shape */
