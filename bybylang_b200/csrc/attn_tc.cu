@@ -660,9 +660,11 @@ static int launch(const kvc::Cache& c, const Params& p, const DeviceInfo& info, 
     if (splits > 1)
         if (int rc = scratch.take(info.device, static_cast<int64_t>(c.n_tokens) * p.q_heads, static_cast<int>(splits), c.head_dim, stream, &part)) return rc;
     cudaLaunchAttribute attr[1];
-    // K and V of a band: about half of the 126 MB L2
+    // K and V of a band: about half of the 126 MB L2; bands of one size, so that none is short
     const int64_t unit_bytes = std::min<int64_t>(span, split_keys) * c.head_dim * 4;
-    const int band = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((64 << 20) / unit_bytes, 1 << 20)));
+    const int64_t kv_units = static_cast<int64_t>(c.n_seqs) * c.kv_heads * splits;
+    const int64_t bands = ceil_div(kv_units, std::max<int64_t>(1, (64 << 20) / unit_bytes));
+    const int band = static_cast<int>(ceil_div(kv_units, bands));
     const cudaLaunchConfig_t cfg = pdl_config(dim3(static_cast<unsigned>(units * splits)), kThreads, C::kSmem, stream, attr);
     BYBYCU_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, maps, c, p, part, split_keys, static_cast<int>(splits), static_cast<int>(tiles), band,
                                        tile_rows, box_slots));

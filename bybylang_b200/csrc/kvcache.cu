@@ -14,8 +14,9 @@ namespace kvc {
 // Of token t at position p: (x, y) -> m (x cos a - y sin a, x sin a + y cos a) for each pair i,
 // a = 2 pi frac(p * turns[i]).  The product is taken in fp64 and only its fraction converted to
 // fp32: an fp32 angle at position 30000 is off by up to 2^-10 rad, which a bf16 key still shows.
-// One block per token: pairs angles once per token (64 fp64 products and sincospif, shared by
-// all heads), then every vector of 8 values of q, k and v.
+// One block per token: its angles once (an fp64 product and sincospif a pair, shared by all heads),
+// then every vector of 8 values of q, k and v, the first of them loaded before the angles are
+// worked out.  Bound by HBM for prompts, by latency for single tokens.
 // ---------------------------------------------------------------------------------------
 struct RopeParams {
     const void *q, *k, *v;
@@ -27,26 +28,35 @@ struct RopeParams {
     float magnitude;
 };
 
-constexpr int kRopeThreads = 256;
+constexpr int kRopeThreads = 128;
 
-template <int N, typename T>
-__device__ __forceinline__ void load_vec(const T* p, float (&x)[N]) {
-    if constexpr (N == 8 && sizeof(T) == 4) {
-        const float4 a = __ldcs(reinterpret_cast<const float4*>(p)), b = __ldcs(reinterpret_cast<const float4*>(p) + 1);
-        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-    } else if constexpr (N == 8) {
-        const uint4 a = __ldcs(reinterpret_cast<const uint4*>(p));
-        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+// VEC values as they lie in memory: loads that are issued long before their values are needed.
+template <typename T, int VEC>
+struct RawVec {
+    static constexpr int kWords = VEC * static_cast<int>(sizeof(T)) / 16;   // 16-byte words of a whole vector
+    uint4 w[kWords > 0 ? kWords : 1];
+    T s[1];
+    __device__ __forceinline__ void load(const T* p) {
+        if constexpr (VEC == 1) {
+            s[0] = *p;
+        } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            x[2 * i] = __uint_as_float(w[i] << 16);
-            x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+            for (int i = 0; i < kWords; ++i) w[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
         }
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) x[i] = static_cast<float>(p[i]);
     }
-}
+    __device__ __forceinline__ void values(float (&x)[VEC]) const {
+        if constexpr (VEC == 1) {
+            x[0] = static_cast<float>(s[0]);
+        } else {
+            const uint32_t* u = reinterpret_cast<const uint32_t*>(w);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                if constexpr (sizeof(T) == 4) x[i] = __uint_as_float(u[i]);
+                else x[i] = __uint_as_float(i & 1 ? u[i / 2] & 0xffff0000u : u[i / 2] << 16);
+            }
+        }
+    }
+};
 
 template <int N>
 __device__ __forceinline__ void store_vec(__nv_bfloat16* p, const float (&x)[N]) {
@@ -62,14 +72,49 @@ __device__ __forceinline__ void store_vec(__nv_bfloat16* p, const float (&x)[N])
     }
 }
 
-// VEC: values of a vector access (8 where the layout allows 16-byte accesses, else 1; a pair of
-// the interleaved layout then takes two).
+// VEC: values of a vector access (8 where the layout allows 16-byte accesses, else 1).  A unit is
+// one vector, or the two that a rotation pairs: i and i + pairs (half layout), or for single
+// values 2i and 2i + 1 (whole vectors of the interleaved layout hold their own pairs).
 template <typename T, int VEC, bool INTERLEAVED>
 __global__ void __launch_bounds__(kRopeThreads) rope_append_kernel(const Cache c, const RopeParams p) {
     __shared__ float s_cos[kMaxHeadDim / 2], s_sin[kMaxHeadDim / 2];
+    constexpr bool kTwo = !INTERLEAVED || VEC == 1;          // a turned unit is two vectors
+    constexpr int kStep = INTERLEAVED && VEC == 1 ? 2 : VEC; // dimensions between turned units
+    constexpr int kBatch = 2;                                // units of a thread in flight
+    const int t = blockIdx.x, D = c.head_dim, R = 2 * p.pairs;
+    const int turned = INTERLEAVED ? R / kStep : p.pairs / VEC, units = turned + (D - R) / VEC;
+    const int qk = (p.q_heads + c.kv_heads) * units, total = qk + c.kv_heads * (D / VEC);
+    struct Unit {
+        RawVec<T, VEC> x, y;
+        int h, d;            // head (q, then k, then v), first dimension
+        bool pair;
+    };
+    const int apart = INTERLEAVED ? 1 : p.pairs;
+    auto fetch = [&](int u, Unit& n) {
+        const T* src;
+        n.pair = false;
+        if (u >= qk) {
+            n.h = p.q_heads + c.kv_heads + (u - qk) / (D / VEC);
+            n.d = (u - qk) % (D / VEC) * VEC;
+            src = static_cast<const T*>(p.v) + t * p.v_token + (n.h - p.q_heads - c.kv_heads) * p.v_head + n.d;
+        } else {
+            const int i = u % units;
+            n.h = u / units;
+            n.pair = i < turned;
+            n.d = n.pair ? i * kStep : R + (i - turned) * VEC;
+            src = (n.h < p.q_heads ? static_cast<const T*>(p.q) + t * p.q_token + n.h * p.q_head
+                                   : static_cast<const T*>(p.k) + t * p.k_token + (n.h - p.q_heads) * p.k_head) + n.d;
+        }
+        n.x.load(src);
+        if (kTwo && n.pair) n.y.load(src + apart);
+    };
     pdl_launch_dependents();
     pdl_wait();
-    const int t = blockIdx.x;
+    // the first units are on their way while the token's place and angles are worked out
+    Unit unit[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i)
+        if (static_cast<int>(threadIdx.x) + i * kRopeThreads < total) fetch(threadIdx.x + i * kRopeThreads, unit[i]);
     const int b = block_seq_of(c, t);
     if (b >= c.n_seqs || t < c.q_start[0]) return;   // a row of no sequence
     const int pos = c.kv_lens[b] - (c.q_start[b + 1] - t);
@@ -90,65 +135,47 @@ __global__ void __launch_bounds__(kRopeThreads) rope_append_kernel(const Cache c
         else if (threadIdx.x == 0) record_device_error(kDevErrPage);
     }
     __syncthreads();
-    // A unit is VEC values, or the two vectors of VEC values that a half-layout rotation pairs.
-    const int D = c.head_dim, R = 2 * p.pairs;
-    constexpr int kU = INTERLEAVED && VEC == 1 ? 2 : VEC;            // values of a turned unit's vector
-    const int turned = INTERLEAVED ? R / kU : p.pairs / VEC;         // turned units of a head
-    const int passed = (D - R) / VEC;
-    const int units = turned + passed;
-    const int qk = (p.q_heads + c.kv_heads) * units;
-    const int total = qk + c.kv_heads * (D / VEC);
-    for (int u = threadIdx.x; u < total; u += kRopeThreads) {
-        if (u >= qk) {   // v
-            const int h = (u - qk) / (D / VEC), d = (u - qk) % (D / VEC) * VEC;
-            if (slot < 0) continue;
-            float x[VEC];
-            load_vec<VEC>(static_cast<const T*>(p.v) + t * p.v_token + h * p.v_head + d, x);
-            store_vec<VEC>(c.v + slot + h * c.head_stride + d, x);
-            continue;
-        }
-        const int h = u / units, i = u % units;
-        const bool is_q = h < p.q_heads;
-        const T* src = is_q ? static_cast<const T*>(p.q) + t * p.q_token + h * p.q_head
-                            : static_cast<const T*>(p.k) + t * p.k_token + (h - p.q_heads) * p.k_head;
-        __nv_bfloat16* dst = is_q ? p.q_out + t * p.o_token + h * p.o_head
-                                  : c.k + slot + (h - p.q_heads) * c.head_stride;
-        if (!is_q && slot < 0) continue;
-        const float live = pos >= 0 ? 1.0f : 0.0f;   // a padding token's q row is zero
-        if (i >= turned) {
-            const int d = R + (i - turned) * VEC;
-            float x[VEC];
-            load_vec<VEC>(src + d, x);
+    auto finish = [&](const Unit& n) {
+        __nv_bfloat16* dst;
+        if (n.h < p.q_heads) dst = p.q_out + t * p.o_token + n.h * p.o_head;
+        else if (slot < 0) return;
+        else if (n.h < p.q_heads + c.kv_heads) dst = c.k + slot + (n.h - p.q_heads) * c.head_stride;
+        else dst = c.v + slot + (n.h - p.q_heads - c.kv_heads) * c.head_stride;
+        float x[VEC], y[VEC];
+        n.x.values(x);
+        if constexpr (kTwo) {
+            if (n.pair) {
+                n.y.values(y);
+                const int i0 = INTERLEAVED ? n.d / 2 : n.d;
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) x[e] = live != 0.0f ? x[e] : 0.0f;
-            store_vec<VEC>(dst + d, x);
-        } else if constexpr (INTERLEAVED) {
-            const int d = i * kU;
-            float x[kU];
-            load_vec<kU>(src + d, x);
-#pragma unroll
-            for (int e = 0; e < kU; e += 2) {
-                const float cs = s_cos[(d + e) / 2], sn = s_sin[(d + e) / 2];
-                const float a = x[e] * cs - x[e + 1] * sn, z = x[e] * sn + x[e + 1] * cs;
-                x[e] = live != 0.0f ? a : 0.0f;
-                x[e + 1] = live != 0.0f ? z : 0.0f;
+                for (int e = 0; e < VEC; ++e) {
+                    const float cs = s_cos[i0 + e], sn = s_sin[i0 + e], a = x[e] * cs - y[e] * sn;
+                    y[e] = x[e] * sn + y[e] * cs;
+                    x[e] = a;
+                }
             }
-            store_vec<kU>(dst + d, x);
-        } else {
-            const int d = i * VEC;
-            float x[VEC], y[VEC];
-            load_vec<VEC>(src + d, x);
-            load_vec<VEC>(src + d + p.pairs, y);
+        } else if (n.pair) {
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                const float cs = s_cos[d + e], sn = s_sin[d + e];
-                const float a = x[e] * cs - y[e] * sn, z = x[e] * sn + y[e] * cs;
-                x[e] = live != 0.0f ? a : 0.0f;
-                y[e] = live != 0.0f ? z : 0.0f;
+            for (int e = 0; e < VEC; e += 2) {
+                const float cs = s_cos[(n.d + e) / 2], sn = s_sin[(n.d + e) / 2], a = x[e] * cs - x[e + 1] * sn;
+                x[e + 1] = x[e] * sn + x[e + 1] * cs;
+                x[e] = a;
             }
-            store_vec<VEC>(dst + d, x);
-            store_vec<VEC>(dst + d + p.pairs, y);
         }
+        if (pos < 0) {   // a padding token's q row is zero
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) x[e] = y[e] = 0.0f;
+        }
+        store_vec<VEC>(dst + n.d, x);
+        if (kTwo && n.pair) store_vec<VEC>(dst + n.d + apart, y);
+    };
+    for (int u = threadIdx.x; u < total; u += kBatch * kRopeThreads) {
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i)
+            if (u + i * kRopeThreads < total) finish(unit[i]);
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i)
+            if (u + (kBatch + i) * kRopeThreads < total) fetch(u + (kBatch + i) * kRopeThreads, unit[i]);
     }
 }
 
