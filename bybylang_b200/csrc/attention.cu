@@ -55,7 +55,7 @@ __global__ void __launch_bounds__(kSimtWarps * 32) attention_simt_kernel(const k
                     dot = fmaf(s_q[warp][d + 2 * e + 1], __uint_as_float(u[e] & 0xffff0000u), dot);
                 }
             }
-            sc = score_log2<MOD>(p, dot, slope, pos - j);
+            sc = score_log2<MOD, true>(p, dot, slope, pos - j);
         }
         float mn = fmaxf(m, sc);
 #pragma unroll

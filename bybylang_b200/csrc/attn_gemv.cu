@@ -347,7 +347,7 @@ __global__ void __launch_bounds__(128) attention_gemv_kernel(const kvc::Cache c,
             for (int n = 0; n < C::kKC / 8; ++n)
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    sc[n][e] = score_log2<true>(p, sc[n][e], slope[e >> 1], row_pos[e >> 1] - (j0 + n * 8 + t4 * 2 + (e & 1)));
+                    sc[n][e] = score_log2<true, F32>(p, sc[n][e], slope[e >> 1], row_pos[e >> 1] - (j0 + n * 8 + t4 * 2 + (e & 1)));
         }
         if (masked) {
 #pragma unroll
