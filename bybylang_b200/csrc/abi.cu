@@ -62,9 +62,7 @@ using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t
                                    const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                    CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
-int encode_tensor_map_2d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, uint64_t inner,
-                         uint64_t outer, uint64_t row_stride_bytes, uint32_t box_inner, uint32_t box_outer,
-                         CUtensorMapSwizzle swizzle, CUtensorMapL2promotion promo) {
+static int encode_tiled_entry(EncodeTiledFn* out) {
     static EncodeTiledFn fn = nullptr;
     if (!fn) {
         cudaDriverEntryPointQueryResult q;
@@ -74,6 +72,15 @@ int encode_tensor_map_2d(CUtensorMap* map, CUtensorMapDataType dtype, const void
             return set_error(BYBYCU_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
         fn = reinterpret_cast<EncodeTiledFn>(p);
     }
+    *out = fn;
+    return BYBYCU_OK;
+}
+
+int encode_tensor_map_2d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, uint64_t inner,
+                         uint64_t outer, uint64_t row_stride_bytes, uint32_t box_inner, uint32_t box_outer,
+                         CUtensorMapSwizzle swizzle, CUtensorMapL2promotion promo) {
+    EncodeTiledFn fn = nullptr;
+    if (int rc = encode_tiled_entry(&fn)) return rc;
     const cuuint64_t dims[2] = {inner, outer};
     const cuuint64_t strides[1] = {row_stride_bytes};
     const cuuint32_t box[2] = {box_inner, box_outer};

@@ -12,9 +12,12 @@
 // While the tensor core works on one tile's O += P V and next S, the other tile's group is at its
 // exponentials: at 128 dimensions a block's two products take the tensor core about as long
 // (2 * 128^3 multiplies at 4096 a cycle) as its 128^2 exponentials take the SM's special-function
-// units (16 a cycle), so neither may wait for the other.  One thread a row took 4800 cycles a pair
-// of blocks (tensor core and special-function units 37% busy each, ncu): the chain scores - maximum
-// - exponentials - probabilities of 128 keys in one thread was longer than the other tile's MMAs.
+// units (16 a cycle), so neither may wait for the other.
+//   Measured: 2 sequences of 4096 tokens, 32 heads of 128, 281 us (980 TFLOP/s); with 8 kv heads
+// 274 us; heads of 64 at half of that rate (the exponentials are the same).  A pair of blocks takes
+// some 3300 cycles where its MMAs alone are 2048: a tile's softmax (1700, issue and latency of four
+// warps on a scheduler) and its own P V and S (1350) follow one another, and only the other tile's
+// run beside them.
 //
 //   * The running maximum is only followed when it grew by more than 2^8: probabilities then stay
 //     below 2^8, with the same relative rounding in bf16 and sums in fp32, and the accumulators in
@@ -36,7 +39,7 @@ namespace bybycu {
 namespace attn {
 namespace tcore {
 
-constexpr int kThreads = 576;   // 112 registers a thread
+constexpr int kThreads = 576;   // 18 warps, five on a quarter of the SM: 96 registers a thread
 constexpr int kLoadWarp = 16, kMmaWarp = 17;
 constexpr int kHalf = 64;       // keys of a softmax thread
 constexpr int kFma = 3;         // of 16 exponentials that the FMA units take over: 0, 2, 4, 5, 7 of 16
@@ -597,14 +600,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
 
 // A bf16 tensor map of `rank` dimensions, the first one dense; strides in elements.
 static int encode_map(CUtensorMap* map, const void* base, int rank, const int64_t* dims, const int64_t* strides, const int* box) {
-    static EncodeTiledFn fn = nullptr;
-    if (!fn) {
-        cudaDriverEntryPointQueryResult q;
-        void* f = nullptr;
-        BYBYCU_CUDA_TRY(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q));
-        if (q != cudaDriverEntryPointSuccess || !f) return set_error(BYBYCU_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
-        fn = reinterpret_cast<EncodeTiledFn>(f);
-    }
+    EncodeTiledFn fn = nullptr;
+    if (int rc = encode_tiled_entry(&fn)) return rc;
     cuuint64_t d[4], st[3];
     cuuint32_t bx[4], es[4];
     for (int i = 0; i < rank; ++i) {

