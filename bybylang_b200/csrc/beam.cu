@@ -136,7 +136,7 @@ __device__ __forceinline__ void warp_merge(const uint64_t* lists, int n_lists, i
 // not below the smallest of these.  After 2, 4, 8, 16 and 32 chunks the same with the r-th best
 // candidates, so that for logits in no particular order some 2 * keep / c elements of the c-th
 // chunks become candidates.  A warp that has more than kSoft cuts them down to its best keep.
-// 256 rows of 128256 bf16 (66 MB) take 48 us with the second kernel, 1.4 TB/s: bound by the
+// 256 rows of 128256 bf16 (66 MB) take 42 us with the second kernel, 1.6 TB/s: bound by the
 // instructions a logit (block-wide bounds met at a barrier every 2048 logits took 61 us, a warp's
 // bound from its own first 256 logits 80 us).
 template <typename T, bool VEC>
@@ -158,33 +158,37 @@ __global__ void __launch_bounds__(kThreads, 4) beam_scan_kernel(const Params p) 
     int* count = s_count + warp;
     // a lane's tokens of the warp's c-th chunk ascend with i
     auto token = [&](int c, int i) { return lo + (c * kWarps + warp) * kChunk + (i / kVec * 32 + lane) * kVec + i % kVec; };
-    auto fetch = [&](int c, uint4 (&raw)[kLoads]) {   // whole vectors only; the ragged end is read by itself
-        if constexpr (VEC) {
+    // chunks of this warp that lie in the slice whole: loaded as vectors ahead of time; the ragged
+    // end is read by itself
+    const int left = hi - lo - warp * kChunk;   // of this warp's part
+    const int whole = VEC && left >= kChunk ? (left - kChunk) / (kWarps * kChunk) + 1 : 0;
+    const T* mine = x + lo + warp * kChunk + lane * kVec;
+    auto fetch = [&](int c, uint4 (&raw)[kLoads]) {
+        if (c < whole) {
 #pragma unroll
             for (int i = 0; i < kLoads; ++i)
-                if (token(c, i * kVec) + kVec <= hi) raw[i] = __ldcs(reinterpret_cast<const uint4*>(x + token(c, i * kVec)));
+                raw[i] = __ldcs(reinterpret_cast<const uint4*>(mine + c * (kWarps * kChunk) + i * 32 * kVec));
         }
     };
     auto unpack = [&](int c, const uint4 (&raw)[kLoads], float (&v)[kItems]) {
+        if (c < whole) {
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            if (VEC && token(c, i * kVec) + kVec <= hi) {
+            for (int i = 0; i < kLoads; ++i) {
                 const uint32_t u[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
 #pragma unroll
                 for (int e = 0; e < kVec; ++e) {
                     if constexpr (sizeof(T) == 4) v[i * kVec + e] = __uint_as_float(u[e % 4]);
                     else v[i * kVec + e] = __uint_as_float(e & 1 ? u[e / 2 % 4] & 0xffff0000u : u[e / 2 % 4] << 16);
                 }
-            } else {
+            }
+        } else {
 #pragma unroll
-                for (int e = 0; e < kVec; ++e) {
-                    const int t = token(c, i * kVec + e);
-                    v[i * kVec + e] = t < hi ? static_cast<float>(x[t]) : -INFINITY;
-                }
+            for (int i = 0; i < kItems; ++i) {
+                const int t = token(c, i);
+                v[i] = t < hi ? static_cast<float>(x[t]) : -INFINITY;
             }
         }
     };
-    const int left = hi - lo - warp * kChunk;   // of this warp's part
     const int chunks = left > 0 ? (left + kWarps * kChunk - 1) / (kWarps * kChunk) : 0;
     uint4 raw[2][kLoads];
 #pragma unroll
@@ -243,7 +247,12 @@ __global__ void __launch_bounds__(kThreads, 4) beam_scan_kernel(const Params p) 
             if (__any_sync(~0u, top >= bound_value)) {
                 uint32_t some = 0;
 #pragma unroll
-                for (int i = 0; i < kItems; ++i) some |= v[i] >= bound_value && token(c, i) < hi ? 1u << i : 0u;
+                for (int i = 0; i < kItems; ++i) some |= v[i] >= bound_value ? 1u << i : 0u;
+                if (c >= whole) {   // not what stands for tokens past the slice
+#pragma unroll
+                    for (int i = 0; i < kItems; ++i)
+                        if (token(c, i) >= hi) some &= ~(1u << i);
+                }
                 while (some) {   // few: read again rather than kept in reach of an index
                     const int t = token(c, __ffs(some) - 1);
                     const uint64_t k = (static_cast<uint64_t>(ordered_bits(static_cast<float>(x[t]))) << 32) | ~static_cast<uint32_t>(t);
@@ -407,7 +416,7 @@ extern "C" int bybycu_beam_select(const void* logits, int logits_dtype, int64_t 
     DeviceInfo info;
     if (int rc = current_device_info(&info)) return rc;
     const int64_t rows = static_cast<int64_t>(groups) * beams;
-    // Slices of whole chunks: two blocks an SM or a few more (1, 2, 4 times as many: 48, 53, 56 us at
+    // Slices of whole chunks: two blocks an SM or a few more (1, 2, 4 times as many: 48, 53, 56 us then, at
     // 256 rows of 128256 bf16), but no more than a warp of the second kernel joins at once.
     constexpr int kPiece = beam::kWarps * beam::kChunk;
     const int chunks = static_cast<int>(ceil_div(vocab, kPiece));
