@@ -225,10 +225,13 @@ __global__ void __launch_bounds__(kThreads, 4) beam_scan_kernel(const Params p) 
                 sum *= ex2((m - top) * kLog2e);
                 m = top;
             }
-            // a NaN or +inf logit makes the sum NaN, which kills the row
-            const float off = m == -INFINITY ? 0.0f : -m * kLog2e;
+            // The difference from the maximum comes before the scaling: it is exact near the maximum,
+            // whatever their size, where the rounding of m * log2e alone would be an exponent of 2^8
+            // and more beside a mask of -1e10, and overflows for the lowest numbers.  A NaN or +inf
+            // logit makes the sum NaN, which kills the row.
+            const float base = m == -INFINITY ? 0.0f : m;
 #pragma unroll
-            for (int i = 0; i < kItems; ++i) sum += ex2(fmaf(v[i], kLog2e, off));   // a place past the slice adds 0
+            for (int i = 0; i < kItems; ++i) sum += ex2((v[i] - base) * kLog2e);   // a place past the slice adds 0
             if (c == 0 && left >= 32 * kVec && (bounded || p.keep <= 32)) {
                 int first = 0;
 #pragma unroll

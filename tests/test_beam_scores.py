@@ -1,0 +1,61 @@
+"""beam_select's scores where a row's logits lie far from zero: masks of large negative finite
+values, offsets, and beams whose own score is a sentinel."""
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from bybylang_b200 import _lib  # noqa: E402
+from bybylang_b200 import kvcache as kv  # noqa: E402
+
+DEV = "cuda:0"
+pytestmark = pytest.mark.gpu
+
+
+def against64(logits, scores, keep, tol=None):
+    """Compares a call with prior + log_softmax in 64 bits, order and scores.  Tolerance: the score
+    is prior + ((x - m) - log(sum)): each of the three operations and the inputs of the last rounds
+    by 2^-24 of a term that is at most |score| + |prior| + log(vocab); the sum's terms are good to 2^-22 (the
+    exponential and its argument), a lane adds at most 16 of them here before some 13 joins, each
+    rounding by 2^-24 of the sum, which moves its logarithm by that much."""
+    got, beam, token = kv.beam_select(logits, scores, keep)
+    torch.cuda.synchronize()
+    assert _lib.device_error() == 0
+    groups, beams = scores.shape
+    x = logits.cpu().double().view(groups, beams, -1)
+    s = scores.cpu().double()[..., None] + torch.log_softmax(x, -1)
+    want, at = torch.sort(s.flatten(1), dim=1, descending=True, stable=True)
+    want, at = want[:, :keep], at[:, :keep]
+    got = got.cpu().double()
+    fixed = 2.0 ** -22 + 29 * 2.0 ** -24
+    bound = fixed + 2.0 ** -22 * (want.abs() + scores.cpu().abs().max().double() + math.log(x.shape[2]))
+    assert torch.isfinite(got).all()
+    assert ((got - want).abs() <= bound).all(), float(((got - want).abs() - bound).max())
+    place = beam.cpu().long() * x.shape[2] + token.cpu().long()
+    mine = torch.gather(s.flatten(1), 1, place)
+    assert ((mine - want).abs() <= bound).all()
+    assert all(len(set(p.tolist())) == keep for p in place)
+    return got, beam.cpu(), token.cpu(), at
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab", [40, 4096, 4099, 128256])
+@pytest.mark.parametrize("mask", [-1e4, -1e9, -1e10, -1e20, -1e30, -2.5e38, "least"])
+def test_finite_masks(mask, vocab, dtype):
+    """Eight free tokens of the vocabulary, the others at a large negative number: most lanes see
+    nothing but masked logits."""
+    g = torch.Generator().manual_seed(vocab)
+    mask = float(torch.finfo(dtype).min) if mask == "least" else mask
+    x = torch.full((6, vocab), mask)
+    for row in range(6):
+        x[row, torch.randperm(vocab, generator=g)[:8]] = 2 * torch.randn(8, generator=g)
+    s = -torch.rand(2, 3, generator=g)
+    x = x.to(dtype).to(DEV)
+    got, beam, token, at = against64(x, s.to(DEV), 8)
+    assert (got > -100).all()
+    # the masked ones come last, by their own order: two free tokens a row at most stand before them
+    y = torch.full((1, vocab), mask)
+    y[0, [vocab // 2, 7]] = torch.tensor([1.0, 3.0])
+    got, beam, token, at = against64(y.to(dtype).to(DEV), torch.zeros(1, 1, device=DEV), 6)
+    assert token[0].tolist() == [7, vocab // 2, 0, 1, 2, 3]
