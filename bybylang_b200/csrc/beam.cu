@@ -1,7 +1,7 @@
 // beam.cu - beam search's selection over beams and vocabulary.
 //
-// score(b, t) = scores[b] + (x[b][t] - lse[b]), lse[b] = m + log(sum_t exp(x[b][t] - m)): every
-// logit is needed once for the sum, and the order of a beam's continuations is the order of its
+// score(b, t) = scores[b] + ((x[b][t] - m[b]) - log(sum_t exp(x[b][t] - m[b]))), m the row's largest:
+// every logit is needed once for the sum, and the order of a beam's continuations is the order of its
 // logits.  So one pass over the logits does both: a block walks one slice of one row, each thread
 // with a running maximum and sum, and collects the logits that can still be among the slice's
 // `keep` largest; a second, small kernel joins the slices of each row and then the beams of each
@@ -334,10 +334,11 @@ __global__ void beam_merge_kernel(const Params p, int buf_keys) {
         float sum = part.x == -INFINITY ? part.y : part.y * ex2((part.x - m) * kLog2e);
 #pragma unroll
         for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-        const float lse = m + logf(sum);
+        // m and log(sum) stay apart: their sum would round at the size of m
+        const float log_sum = logf(sum);
         uint64_t* list = s_list + b * K;
         // every continuation of a dead beam scores -inf: its tokens count in their own order
-        const bool dead = !(fabsf(lse) < INFINITY) || isnan(prior) || prior == -INFINITY;
+        const bool dead = !(fabsf(m) < INFINITY) || !(sum < INFINITY) || isnan(prior) || prior == -INFINITY;
         if (dead) {
             for (int i = lane; i < K; i += 32)
                 list[i] = i < p.vocab ? (static_cast<uint64_t>(ordered_bits(-INFINITY)) << 32) | ~static_cast<uint32_t>(i) : 0;
@@ -347,7 +348,7 @@ __global__ void beam_merge_kernel(const Params p, int buf_keys) {
         __syncwarp();
         for (int i = lane; i < K; i += 32) {
             const uint64_t k = list[i];
-            float sc = dead ? -INFINITY : prior + (from_ordered(static_cast<uint32_t>(k >> 32)) - lse);
+            float sc = dead ? -INFINITY : prior + ((from_ordered(static_cast<uint32_t>(k >> 32)) - m) - log_sum);
             if (isnan(sc)) sc = -INFINITY;
             s_final[b * K + i] = k ? (static_cast<uint64_t>(ordered_bits(sc)) << 32) | ~static_cast<uint32_t>(b * kMaxKeep + i) : 0;
         }

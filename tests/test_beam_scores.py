@@ -59,3 +59,19 @@ def test_finite_masks(mask, vocab, dtype):
     y[0, [vocab // 2, 7]] = torch.tensor([1.0, 3.0])
     got, beam, token, at = against64(y.to(dtype).to(DEV), torch.zeros(1, 1, device=DEV), 6)
     assert token[0].tolist() == [7, vocab // 2, 0, 1, 2, 3]
+
+
+@pytest.mark.parametrize("vocab", [1000, 32768, 128256])
+@pytest.mark.parametrize("offset", [0.0, 50.0, -200.0, 200.0, -1000.0, 1000.0, -10000.0, 10000.0])
+def test_offsets(offset, vocab):
+    """Logits that share an offset have the same log-softmax."""
+    g = torch.Generator().manual_seed(int(abs(offset)) + vocab)
+    x = (2 * torch.randn(8, vocab, generator=g) + offset).to(DEV)
+    s = -4 * torch.rand(2, 4, generator=g)
+    against64(x, s.to(DEV), 16)
+
+
+def test_offset_rows_in_bf16():
+    g = torch.Generator().manual_seed(1)
+    x = 2 * torch.randn(8, 32768, generator=g) + torch.tensor([0.0, 100, -100, 200, -200, 30, 500, -500])[:, None]
+    against64(x.to(torch.bfloat16).to(DEV), (-4 * torch.rand(2, 4, generator=g)).to(DEV), 16)
