@@ -1,6 +1,7 @@
 // attention.cu - attention of new tokens over a paged cache: the checks, the choice of a route,
 // and the SIMT route (one warp a query row, fp32 throughout).
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 
 #include "attention.cuh"
@@ -132,10 +133,12 @@ extern "C" int bybycu_paged_attention(const bybycu_paged_kv* kv, const bybycu_at
         !kvc::strides_ok(a->q_token_stride, a->q_head_stride, a->q_heads, c.head_dim, 8) ||
         !kvc::strides_ok(a->out_token_stride, a->out_head_stride, a->q_heads, c.head_dim, oal))
         return set_error(BYBYCU_ERR_ARGS, "paged_attention: q and out need 16-byte aligned vectors that do not overlap");
+    // finite even where the quotient overflows: a score of 0 stays 0 under the smallest cap
+    const float cap_in = a->softcap > 0.0f ? std::clamp(a->scale / a->softcap, -FLT_MAX / 4, FLT_MAX / 4) : 0.0f;
     const attn::Params p{static_cast<const __nv_bfloat16*>(a->q), a->out, a->q_token_stride, a->q_head_stride,
                          a->out_token_stride, a->out_head_stride, a->slopes, a->prefix_lens, a->q_heads,
                          a->q_heads / c.kv_heads, a->max_q, a->max_kv, a->window, a->scale * attn::kLog2e, a->softcap,
-                         a->softcap > 0.0f ? 2.0f * attn::kLog2e * (a->scale / a->softcap) : 0.0f, a->softcap * attn::kLog2e};
+                         cap_in, 2.0f * attn::kLog2e * cap_in, a->softcap * attn::kLog2e};
     const bool mod = a->softcap > 0.0f || a->slopes, f32 = a->out_dtype == BYBYCU_DT_F32;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (a->route == BYBYCU_ROUTE_SIMT) return attn::launch_simt(c, p, mod, f32, s);

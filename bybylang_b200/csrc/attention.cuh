@@ -16,7 +16,8 @@ struct Params {
     const float* slopes;
     const int32_t* prefix;
     int32_t q_heads, group, max_q, max_kv, window;   // group: query heads a kv head
-    float scale_log2, cap, cap_in, cap_out;          // scale * log2(e); softcap; 2 log2(e) scale / softcap; softcap * log2(e)
+    // scale * log2(e); softcap; scale / softcap; 2 log2(e) scale / softcap; softcap * log2(e)
+    float scale_log2, cap, cap_in, cap_ex, cap_out;
 };
 
 // One sequence of the batch as a kernel reads it.  rows and kv are what may be touched: never past
@@ -65,40 +66,50 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     return d;
 }
 
-// cap * tanh(y) of two scores in units of log2, y = raw * scale / cap: tanh(y) = 1 - 2 / (1 + e^2y)
-// with the hardware's exponential and one reciprocal for both.  The absolute error is a few
-// 2^-24 times the cap.  2 y log2(e) is held below 60, where tanh is 1 in fp32, so that the
-// product of the two denominators stays finite.
-__device__ __forceinline__ float2 capped_log2(const Params& p, float raw0, float raw1) {
-    const float a = 1.0f + ex2(min_nan(raw0 * p.cap_in, 60.0f)), b = 1.0f + ex2(min_nan(raw1 * p.cap_in, 60.0f));
+// A capped score: cap * tanh(y) in units of log2, y = raw * scale / cap.
+//   plain:  cap * (1 - 2 / (1 + e^2y)), off by some 1e-7 of the cap wherever y is.  For a bf16
+//           output and caps up to kCapPlain that is 3e-5 of a score, far below the rounding of a
+//           probability; at a cap of 1e6 it made probabilities wrong by 9%
+//   exact:  for |y| < 0.6  s * (1 + y^2 P(y^2)), s the score without a cap, P of degree 4 (tanh(y)
+//           to 4.2e-9 of itself, a Chebyshev fit), and the plain form above, where it is good to
+//           2^-22 of itself: off by a few 2^-24 of the score, however large the cap.
+constexpr float kCapPlain = 256.0f;
+constexpr float kCapBend = 0.6f;   // where the two forms of `exact` meet
+constexpr float kCapP0 = -0.333332956f, kCapP1 = 0.133318797f, kCapP2 = -0.0537803993f, kCapP3 = 0.0207851473f, kCapP4 = -0.00588323316f;
+
+__device__ __forceinline__ float rcp(float x) {
     float r;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(a * b));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float capped_plain(const Params& p, float raw) {
+    return fmaf(-2.0f * p.cap_out, rcp(1.0f + ex2(raw * p.cap_ex)), p.cap_out);
+}
+__device__ __forceinline__ float capped_small(const Params& p, float raw) {
+    const float y = raw * p.cap_in, z = y * y, s = raw * p.scale_log2;
+    return fmaf(s * z, fmaf(fmaf(fmaf(fmaf(kCapP4, z, kCapP3), z, kCapP2), z, kCapP1), z, kCapP0), s);
+}
+__device__ __forceinline__ float capped_exact(const Params& p, float raw) {
+    const float small = capped_small(p, raw), large = capped_plain(p, raw);
+    return fabsf(raw * p.cap_in) < kCapBend ? small : large;   // a NaN goes through
+}
+// The plain form of two scores with one reciprocal.  The exponents are held below 60, where tanh is
+// 1 in fp32, so that the product of the two denominators stays finite.
+__device__ __forceinline__ float2 capped_plain(const Params& p, float raw0, float raw1) {
+    const float a = 1.0f + ex2(min_nan(raw0 * p.cap_ex, 60.0f)), b = 1.0f + ex2(min_nan(raw1 * p.cap_ex, 60.0f));
+    const float r = rcp(a * b);
     return make_float2(fmaf(-2.0f * p.cap_out, r * b, p.cap_out), fmaf(-2.0f * p.cap_out, r * a, p.cap_out));
 }
 
-// The same of one score, for an fp32 output: below y = 0.6, where the difference from 1 loses the
-// digits of a small result, tanh(y) = y + y^3 P(y^2) with P of degree 4 (relative error 3e-9, a
-// Chebyshev fit).  With scores of order 1 under a cap of 30 the output was off by 1.4e-6 without it
-// and is by 2e-7.
-__device__ __forceinline__ float capped_log2_exact(const Params& p, float raw) {
-    const float y = raw * p.cap_in * 0.34657359f, z = y * y;   // cap_in holds 2 log2(e)
-    float t = fmaf(-0.00588323316f, z, 0.0207851473f);
-    t = fmaf(t, z, -0.0537803993f);
-    t = fmaf(t, z, 0.133318797f);
-    t = fmaf(t, z, -0.333332956f);
-    const float small = p.cap_out * fmaf(t, y * z, y);
-    return z < 0.36f ? small : capped_log2(p, raw, 0.0f).x;
-}
-
-// The score of a pair in units of log2: raw = q . k, MOD: a cap (EXACT: for an fp32 output) and /
-// or distance slopes.
+// The score of a pair in units of log2: raw = q . k, MOD: a cap (EXACT: for an fp32 output) and / or
+// distance slopes.
 template <bool MOD, bool EXACT>
 __device__ __forceinline__ float score_log2(const Params& p, float raw, float slope_log2, int distance) {
     if constexpr (!MOD) {
         return raw * p.scale_log2;
     } else {
         float s = raw * p.scale_log2;
-        if (p.cap > 0.0f) s = EXACT ? capped_log2_exact(p, raw) : capped_log2(p, raw, 0.0f).x;
+        if (p.cap > 0.0f) s = EXACT || p.cap > kCapPlain ? capped_exact(p, raw) : capped_plain(p, raw);
         return s - slope_log2 * static_cast<float>(distance < 0 ? -distance : distance);
     }
 }

@@ -447,11 +447,26 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
                             for (int e = 0; e < 32; ++e)
                                 if (e < lo || e >= hi) sc[e] = 0u;
                         }
+                        if (p.cap <= kCapPlain) {
 #pragma unroll
-                        for (int e = 0; e < 32; e += 2) {
-                            const float2 t = capped_log2(p, __uint_as_float(sc[e]), __uint_as_float(sc[e + 1]));
-                            sc[e] = __float_as_uint(t.x);
-                            sc[e + 1] = __float_as_uint(t.y);
+                            for (int e = 0; e < 32; e += 2) {
+                                const float2 t = capped_plain(p, __uint_as_float(sc[e]), __uint_as_float(sc[e + 1]));
+                                sc[e] = __float_as_uint(t.x);
+                                sc[e + 1] = __float_as_uint(t.y);
+                            }
+                        } else {
+                            // under such a cap hardly a score comes to where it bends: a warp whose
+                            // 32 rows have none takes the polynomial alone
+                            float largest = 0.0f;
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) largest = fmaxf(largest, fabsf(__uint_as_float(sc[e])));
+                            if (__all_sync(~0u, largest * fabsf(p.cap_in) < kCapBend)) {
+#pragma unroll
+                                for (int e = 0; e < 32; ++e) sc[e] = __float_as_uint(capped_small(p, __uint_as_float(sc[e])));
+                            } else {
+#pragma unroll
+                                for (int e = 0; e < 32; ++e) sc[e] = __float_as_uint(capped_exact(p, __uint_as_float(sc[e])));
+                            }
                         }
                     } else {
 #pragma unroll
