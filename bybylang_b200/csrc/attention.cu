@@ -131,7 +131,7 @@ extern "C" int bybycu_paged_attention(const bybycu_paged_kv* kv, const bybycu_at
     const int oal = a->out_dtype == BYBYCU_DT_F32 ? 4 : 8;   // 16-byte output vectors
     if (!kvc::aligned(a->q, 16) || !kvc::aligned(a->out, 16) || !kvc::aligned(a->slopes, 4) || !kvc::aligned(a->prefix_lens, 4) ||
         !kvc::strides_ok(a->q_token_stride, a->q_head_stride, a->q_heads, c.head_dim, 8) ||
-        !kvc::strides_ok(a->out_token_stride, a->out_head_stride, a->q_heads, c.head_dim, oal))
+        !kvc::out_strides_ok(a->out_token_stride, a->out_head_stride, c.n_tokens, a->q_heads, c.head_dim, oal))
         return set_error(BYBYCU_ERR_ARGS, "paged_attention: q and out need 16-byte aligned vectors that do not overlap");
     // finite even where the quotient overflows: a score of 0 stays 0 under the smallest cap
     const float cap_in = a->softcap > 0.0f ? std::clamp(a->scale / a->softcap, -FLT_MAX / 4, FLT_MAX / 4) : 0.0f;

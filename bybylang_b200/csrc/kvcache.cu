@@ -297,7 +297,7 @@ int bybycu_rope_append(const bybycu_paged_kv* kv, const bybycu_rope* r, void* st
     if (!kvc::strides_ok(r->q_token_stride, r->q_head_stride, r->q_heads, c.head_dim, 1) ||
         !kvc::strides_ok(r->k_token_stride, r->k_head_stride, c.kv_heads, c.head_dim, 1) ||
         !kvc::strides_ok(r->v_token_stride, r->v_head_stride, c.kv_heads, c.head_dim, 1) ||
-        !kvc::strides_ok(r->out_token_stride, r->out_head_stride, r->q_heads, c.head_dim, 1))
+        !kvc::out_strides_ok(r->out_token_stride, r->out_head_stride, c.n_tokens, r->q_heads, c.head_dim, 1))
         return set_error(BYBYCU_ERR_ARGS, "rope_append: negative or overlapping strides");
     const kvc::RopeParams p{r->q, r->k, r->v, static_cast<__nv_bfloat16*>(r->q_out),
                             r->q_token_stride, r->q_head_stride, r->k_token_stride, r->k_head_stride,

@@ -65,6 +65,14 @@ inline int check_cache(const bybycu_paged_kv* kv, const char* op, Cache* c) {
 inline bool strides_ok(int64_t token, int64_t head, int heads, int dim, int align) {
     return token >= 0 && head >= 0 && token % align == 0 && head % align == 0 && (heads == 1 || head >= dim);
 }
+// The same of an output: no two of its vectors may share an element, whichever of tokens and heads
+// lies inside the other.
+inline bool out_strides_ok(int64_t token, int64_t head, int tokens, int heads, int dim, int align) {
+    if (!strides_ok(token, head, heads, dim, align)) return false;
+    if (heads == 1) return tokens == 1 || token >= dim;
+    if (tokens == 1 || (token >= dim && (head - dim) / (tokens - 1) >= token)) return true;
+    return token >= dim && (token - dim) / (heads - 1) >= head;
+}
 
 // Number of the n ends q_start[1..n] that are <= t, counted by a whole block (every thread
 // calls): the sequence of token t, n_seqs when it belongs to none.  The loads of one round are
