@@ -284,7 +284,7 @@ int bybycu_rope_append(const bybycu_paged_kv* kv, const bybycu_rope* r, void* st
     if (r->in_dtype != BYBYCU_DT_F32 && r->in_dtype != BYBYCU_DT_BF16)
         return set_error(BYBYCU_ERR_ARGS, "rope_append: element type must be F32 or BF16");
     if (r->reserved) return set_error(BYBYCU_ERR_ARGS, "rope_append: reserved fields must be 0");
-    if (r->q_heads <= 0 || r->q_heads > 65535 || c.kv_heads > 65535 || r->pairs < 0 || 2 * r->pairs > c.head_dim)
+    if (r->q_heads <= 0 || r->q_heads > 65535 || c.kv_heads > 65535 || r->pairs < 0 || r->pairs > c.head_dim / 2)
         return set_error(BYBYCU_ERR_SHAPE, "rope_append: %d query heads, %d pairs of a head of %d", r->q_heads, r->pairs,
                          c.head_dim);
     if (c.n_tokens == 0 || c.n_seqs == 0) return BYBYCU_OK;

@@ -45,3 +45,10 @@ def test_strides_of_one_token_and_one_head():
     refused(lib.bybycu_paged_attention(cache(kv_heads=1), attention(q_heads=1, out_token_stride=0, out_head_stride=0), None), _lib.ERR_ARGS, "overlap")
     refused(lib.bybycu_paged_attention(cache(n_tokens=1), attention(out_token_stride=0, out_head_stride=0), None), _lib.ERR_ARGS, "overlap")
     refused(lib.bybycu_paged_attention(cache(n_tokens=1), attention(out_token_stride=0, q=0), None), _lib.ERR_ARGS, "missing")
+
+
+@no_device
+@pytest.mark.parametrize("pairs", [33, 1 << 30, (1 << 30) + 16, (1 << 31) - 1])
+def test_pairs_beyond_the_head(pairs):
+    """2 * pairs may not wrap around to a number that fits."""
+    refused(_lib.load().bybycu_rope_append(cache(), rope(pairs=pairs), None), _lib.ERR_SHAPE, "pairs")
