@@ -52,13 +52,16 @@ def _refuse(code: int, message: str):
 
 
 def _stream(op: str, device: int, stream) -> int:
-    """The raw stream of a call on `device`, which has to be the current one."""
+    """The raw stream of a call on `device`, which has to be the current one and the stream's (the
+    default stream has one handle on every device)."""
     import torch
-    if stream is not None:
-        return stream.cuda_stream
     if torch._C._cuda_getDevice() != device:
         _refuse(_lib.ERR_ARGS, f"{op}: the tensors are on cuda:{device}, the current device is cuda:{torch.cuda.current_device()}")
-    return torch._C._cuda_getCurrentRawStream(device)
+    if stream is None:
+        return torch._C._cuda_getCurrentRawStream(device)
+    if stream.device_index != device:
+        _refuse(_lib.ERR_ARGS, f"{op}: the stream is on cuda:{stream.device_index}, the tensors are on cuda:{device}")
+    return stream.cuda_stream
 
 
 def _paged(op: str, n_tokens: int, k_cache, v_cache, page_table, q_start, kv_lens):
