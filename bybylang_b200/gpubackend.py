@@ -275,6 +275,17 @@ def _stream_ptr(stream) -> C.c_void_p:
     return C.c_void_p(s.cuda_stream)
 
 
+def _output(shape, dtype, device, stream):
+    """The output of a call that runs on `stream` (None: the current one).  It comes from that
+    stream's memory: a block of the current stream's may still be in use by work queued there, which
+    the other stream does not wait for."""
+    import torch
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=device)
+
+
 def tile_gemm(fmt: int, x, packed, out, *, M: int, K: int, N: int, scale_base: int = 0, lut=None,
               lut_base: int = 0, route: int = _lib.ROUTE_AUTO, stream=None):
     """out[M, N] = x[M, K] * dequant(W)^T for one OP_TILE_GEMM on device tensors.

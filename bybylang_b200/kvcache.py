@@ -13,6 +13,10 @@ Tensors are torch device tensors, every call is asynchronous on `stream` (defaul
 one) and there is no CPU fallback: a call that cannot run raises ``BybyCudaError``.  Page ids and
 lengths live on the device; the kernels check them and report through ``_lib.device_error()``.
 
+With `stream` given the caller orders it after the stream that made the inputs, and keeps the inputs
+until the work is done.  An output that the call allocates belongs to `stream`; one that is used on
+another stream afterwards needs that stream to wait, and ``record_stream`` before it is dropped.
+
 A batch is three int32 device tensors: ``page_table`` [sequences, pages], ``q_start``
 [sequences + 1] (sequence b's new tokens are rows q_start[b] .. q_start[b+1]) and ``kv_lens``
 [sequences] (tokens in the cache, the new ones included).
@@ -26,7 +30,7 @@ import struct
 
 from . import _lib
 from ._lib import BybyCudaError, check, load
-from .gpubackend import _dtype_code
+from .gpubackend import _dtype_code, _output
 
 # A decode step makes several of these calls a layer, so what a call costs the host counts: the
 # argument structs of include/bybycuda.h are packed in one go (bybycu_paged_kv, bybycu_rope,
@@ -165,8 +169,9 @@ def rope_append(q, k, v, k_cache, v_cache, page_table, q_start, kv_lens, turns, 
     qs = _heads("rope_append", "q", q, T, hq, dim, dev, None)
     ks = _heads("rope_append", "k", k, T, hk, dim, dev, dtype)
     vs = _heads("rope_append", "v", v, T, hk, dim, dev, dtype)
+    raw = _stream("rope_append", dev, stream)
     if q_out is None:
-        q_out = torch.empty((T, hq, dim), dtype=torch.bfloat16, device=q.device)
+        q_out = _output((T, hq, dim), torch.bfloat16, q.device, stream)
         os_ = hq * dim, dim
     else:
         os_ = _heads("rope_append", "q_out", q_out, T, hq, dim, dev, torch.bfloat16)
@@ -175,7 +180,7 @@ def rope_append(q, k, v, k_cache, v_cache, page_table, q_start, kv_lens, turns, 
                  _vector("rope_append", "turns", turns, pairs, torch.float64, dev),
                  _vector("rope_append", "positions", positions, T, torch.int32, dev), _dtype_code(q), hq, pairs,
                  _LAYOUTS[layout], magnitude, 0)
-    check(_call("bybycu_rope_append")(kv, args, _stream("rope_append", dev, stream)))
+    check(_call("bybycu_rope_append")(kv, args, raw))
     return q_out
 
 
@@ -196,15 +201,16 @@ def paged_attention(q, k_cache, v_cache, page_table, q_start, kv_lens, *, max_q:
     T, hq, _ = q.shape
     kv, dev, n_seqs, _, dim = _paged("paged_attention", T, k_cache, v_cache, page_table, q_start, kv_lens)
     qs = _heads("paged_attention", "q", q, T, hq, dim, dev, torch.bfloat16)
+    raw = _stream("paged_attention", dev, stream)
     if out is None:
-        out = torch.empty((T, hq, dim), dtype=torch.bfloat16 if out_dtype is None else out_dtype, device=q.device)
+        out = _output((T, hq, dim), torch.bfloat16 if out_dtype is None else out_dtype, q.device, stream)
         os_ = hq * dim, dim
     else:
         os_ = _heads("paged_attention", "out", out, T, hq, dim, dev, out_dtype)
     args = _ATTENTION(q.data_ptr(), out.data_ptr(), *qs, *os_, _vector("paged_attention", "slopes", slopes, hq, torch.float32, dev),
                       _vector("paged_attention", "prefix_lens", prefix_lens, n_seqs, torch.int32, dev), _dtype_code(out), hq,
                       max_q, max_kv, window, route, dim ** -0.5 if scale is None else scale, softcap)
-    check(_call("bybycu_paged_attention")(kv, args, _stream("paged_attention", dev, stream)))
+    check(_call("bybycu_paged_attention")(kv, args, raw))
     return out
 
 
@@ -255,12 +261,12 @@ def beam_select(logits, scores, keep: int, *, stream=None):
     if scores.dtype != torch.float32 or not scores.is_contiguous() or dev < 0 or scores.get_device() != dev or (vocab > 1 and one != 1):
         _refuse(_lib.ERR_ARGS, "beam_select: scores must be contiguous float32, the rows of logits dense, both on the device")
     groups, beams = scores.shape
-    best = torch.empty((groups, keep), dtype=torch.float32, device=logits.device)
-    which = torch.empty((2, groups, keep), dtype=torch.int32, device=logits.device)
+    raw = _stream("beam_select", dev, stream)
+    best = _output((groups, keep), torch.float32, logits.device, stream)
+    which = _output((2, groups, keep), torch.int32, logits.device, stream)
     at = which.data_ptr()
     check(_call("bybycu_beam_select")(logits.data_ptr(), _dtype_code(logits), stride if rows > 1 else max(1, vocab), scores.data_ptr(),
-                                      groups, beams, vocab, keep, best.data_ptr(), at, at + 4 * groups * keep,
-                                      _stream("beam_select", dev, stream)))
+                                      groups, beams, vocab, keep, best.data_ptr(), at, at + 4 * groups * keep, raw))
     beam, token = which.unbind(0)
     return best, beam, token
 
