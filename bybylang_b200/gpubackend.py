@@ -346,7 +346,7 @@ class Q4B32Weights:
         import torch
         M = x.shape[0]
         if out is None:
-            out = torch.empty(M, self.N, dtype=torch.float32, device=x.device)
+            out = _output((M, self.N), torch.float32, x.device, stream)
         return tile_gemm(TileFormatQ4B32, x, self.packed, out, M=M, K=self.K, N=self.N,
                          scale_base=self.scale_base, route=route, stream=stream)
 
@@ -597,7 +597,7 @@ class Q4AsymWeights:
         import torch
         M = x.shape[0]
         if out is None:
-            out = torch.empty(M, self.N, dtype=torch.float32, device=x.device)
+            out = _output((M, self.N), torch.float32, x.device, stream)
         call("bybycu_matmul_q4", _ptr(x), _ptr(self.wq), _ptr(self.scales), _ptr(self.zeros), _ptr(out), M, self.K,
              self.N, self.group_size, self.n_groups, int(route), _stream_ptr(stream))
         return out

@@ -71,3 +71,33 @@ def test_outputs_come_from_the_stream_that_writes_them(name):
     out.record_stream(torch.cuda.current_stream())
     torch.cuda.synchronize()
     assert _lib.device_error() == 0
+
+
+def weights(kind):
+    from bybylang_b200 import gpubackend as gb
+    gb.ensureGpuInit(gb.GpuBackend.gbCuda, 0)
+    g = torch.Generator().manual_seed(4)
+    wq = torch.randint(0, 256, (512, 128), generator=g, dtype=torch.uint8)
+    if kind == "Q4B32":
+        return gb.Q4B32Weights(wq, torch.full((512, 8), 0.05).to(torch.float16), device=DEV)
+    return gb.Q4AsymWeights(wq, torch.full((512, 8), 0.05), torch.full((512, 8), 7.5), K=256, group_size=32, device=DEV)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["Q4B32", "Q4"])
+def test_projections_come_from_the_stream_that_writes_them(kind):
+    w = weights(kind)
+    x = torch.randn(4, 256, generator=torch.Generator().manual_seed(5)).to(DEV)
+    want = w.matmul(x).clone()
+    size = 4 * 512 * 4
+    at = freed_block(size)
+    out = w.matmul(x)
+    assert out.data_ptr() == at
+    del out
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    at = freed_block(size)
+    out = w.matmul(x, stream=s)
+    assert out.data_ptr() != at
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(out, want)
