@@ -133,11 +133,15 @@ extern "C" int bybycu_paged_attention(const bybycu_paged_kv* kv, const bybycu_at
         !kvc::strides_ok(a->q_token_stride, a->q_head_stride, a->q_heads, c.head_dim, 8) ||
         !kvc::out_strides_ok(a->out_token_stride, a->out_head_stride, c.n_tokens, a->q_heads, c.head_dim, oal))
         return set_error(BYBYCU_ERR_ARGS, "paged_attention: q and out need 16-byte aligned vectors that do not overlap");
+    // no sequence has more new tokens than there are; a tile's rows (token, head of a group) are counted in 32 bits
+    const int max_q = std::min(a->max_q, c.n_tokens);
+    if (static_cast<int64_t>(max_q) * (a->q_heads / c.kv_heads) > INT32_MAX - 256)
+        return set_error(BYBYCU_ERR_SHAPE, "paged_attention: %d new tokens of %d heads a kv head: 2^31 rows or more", max_q, a->q_heads / c.kv_heads);
     // finite even where the quotient overflows: a score of 0 stays 0 under the smallest cap
     const float cap_in = a->softcap > 0.0f ? std::clamp(a->scale / a->softcap, -FLT_MAX / 4, FLT_MAX / 4) : 0.0f;
     const attn::Params p{static_cast<const __nv_bfloat16*>(a->q), a->out, a->q_token_stride, a->q_head_stride,
                          a->out_token_stride, a->out_head_stride, a->slopes, a->prefix_lens, a->q_heads,
-                         a->q_heads / c.kv_heads, a->max_q, a->max_kv, a->window, a->scale * attn::kLog2e, a->softcap,
+                         a->q_heads / c.kv_heads, max_q, a->max_kv, a->window, a->scale * attn::kLog2e, a->softcap,
                          cap_in, 2.0f * attn::kLog2e * cap_in, a->softcap * attn::kLog2e};
     const bool mod = a->softcap > 0.0f || a->slopes, f32 = a->out_dtype == BYBYCU_DT_F32;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -150,7 +154,7 @@ extern "C" int bybycu_paged_attention(const bybycu_paged_kv* kv, const bybycu_at
     // sequences of 4096 keys, 8 kv heads of 128, at 16, 32, 64 and 128 rows 51, 64, 88, 153 us on
     // the GEMV and 43, 46, 51, 61 on the tensor cores; heads of 64 33, 41, 53, 93 and 37, 39, 43,
     // 53; one sequence of 2048 15, 17, 21, 23 and 19, 19, 20, 23.
-    if (a->route == BYBYCU_ROUTE_TC || (a->route == BYBYCU_ROUTE_AUTO && tc && static_cast<int64_t>(a->max_q) * p.group > 32))
+    if (a->route == BYBYCU_ROUTE_TC || (a->route == BYBYCU_ROUTE_AUTO && tc && static_cast<int64_t>(max_q) * p.group > 32))
         return attn::launch_tc_attention(c, p, mod, s);
     return attn::launch_gemv(c, p, f32, s);
 }

@@ -52,3 +52,10 @@ def test_strides_of_one_token_and_one_head():
 def test_pairs_beyond_the_head(pairs):
     """2 * pairs may not wrap around to a number that fits."""
     refused(_lib.load().bybycu_rope_append(cache(), rope(pairs=pairs), None), _lib.ERR_SHAPE, "pairs")
+
+
+@no_device
+def test_launches_past_32_bits():
+    lib, wide = _lib.load(), dict(q_token_stride=1 << 21, out_token_stride=1 << 21)
+    one = dict(kv_heads=1, n_tokens=1 << 16)
+    refused(lib.bybycu_paged_attention(cache(**one), attention(q_heads=1 << 15, max_q=1 << 16, **wide), None), _lib.ERR_SHAPE, "2^31 rows")
