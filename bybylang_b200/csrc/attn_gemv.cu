@@ -131,7 +131,7 @@ struct GemvCfg {
 // granules at a time and a batch ahead, so that no copy waits for the page table.
 template <int HD, int WM, bool F32, bool P16>
 __global__ void __launch_bounds__(128) attention_gemv_kernel(const kvc::Cache c, const Params p, const Partials part,
-                                                             int split_keys, int row_tiles, int cluster) {
+                                                             int split_keys, int tile0, int row_tiles, int cluster) {
     using C = GemvCfg<HD, WM>;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ float s_m[4][16], s_l[4][16];
@@ -140,7 +140,7 @@ __global__ void __launch_bounds__(128) attention_gemv_kernel(const kvc::Cache c,
     pdl_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
     const int wm = warp % WM, wk = warp / WM;
-    const int kvh = blockIdx.y / row_tiles, first_row = blockIdx.y % row_tiles * (16 * WM), b = blockIdx.z, split = blockIdx.x;
+    const int kvh = blockIdx.y / row_tiles, first_row = (tile0 + blockIdx.y % row_tiles) * (16 * WM), b = blockIdx.z, split = blockIdx.x;
     const Seq s = load_seq(c, p, b);
     const int rows = min(16 * WM, s.rows * p.group - first_row);
     if (rows <= 0) return;   // every CTA of a cluster has the same rows
@@ -646,8 +646,9 @@ static int launch_gemv_tile(const kvc::Cache& c, const Params& p, const DeviceIn
     });
     if (prep[info.device] != cudaSuccess) return cuda_fail(prep[info.device], "attention_gemv_kernel shared memory");
     const int row_tiles = static_cast<int>(ceil_div(static_cast<int64_t>(p.max_q) * p.group, 16 * WM));
-    if (static_cast<int64_t>(row_tiles) * c.kv_heads > 65535 || c.n_seqs > 65535)
-        return set_error(BYBYCU_ERR_SHAPE, "paged_attention: %d sequences, %d kv heads, %d new tokens", c.n_seqs, c.kv_heads, p.max_q);
+    // a launch's grid has 65535 rows and layers at most
+    constexpr int kGrid = 65535;
+    if (c.kv_heads > kGrid) return set_error(BYBYCU_ERR_SHAPE, "paged_attention: %d kv heads", c.kv_heads);
     const int64_t units = static_cast<int64_t>(row_tiles) * c.kv_heads * c.n_seqs;
     const int slots = info.sm_count * std::max(1, std::min(3, static_cast<int>(227 * 1024 / (C::kSmem + 2048))));
     const int64_t span = longest_span(p, 16 * WM);
@@ -668,15 +669,27 @@ static int launch_gemv_tile(const kvc::Cache& c, const Params& p, const DeviceIn
     if (splits > 1 && !cluster)
         if (int rc = scratch.take(info.device, static_cast<int64_t>(c.n_tokens) * p.q_heads, splits, c.head_dim, stream, &part)) return rc;
     cudaLaunchAttribute attr[2];
-    cudaLaunchConfig_t cfg = pdl_config(dim3(static_cast<unsigned>(splits), static_cast<unsigned>(row_tiles * c.kv_heads),
-                                             static_cast<unsigned>(c.n_seqs)), 128, C::kSmem, stream, attr);
-    if (cluster) {
-        attr[1].id = cudaLaunchAttributeClusterDimension;
-        attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
-        attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-        cfg.numAttrs = 2;
+    const int tiles_step = std::min(row_tiles, kGrid / c.kv_heads);
+    for (int64_t seq0 = 0; seq0 < c.n_seqs; seq0 += kGrid) {
+        kvc::Cache cc = c;   // the sequences from seq0 on
+        Params pp = p;
+        cc.page_table += seq0 * c.table_stride;
+        cc.q_start += seq0;
+        cc.kv_lens += seq0;
+        if (pp.prefix) pp.prefix += seq0;
+        for (int tile0 = 0; tile0 < row_tiles; tile0 += tiles_step) {
+            const int tiles = std::min(tiles_step, row_tiles - tile0);
+            cudaLaunchConfig_t cfg = pdl_config(dim3(static_cast<unsigned>(splits), static_cast<unsigned>(tiles * c.kv_heads),
+                                                     static_cast<unsigned>(std::min<int64_t>(kGrid, c.n_seqs - seq0))), 128, C::kSmem, stream, attr);
+            if (cluster) {
+                attr[1].id = cudaLaunchAttributeClusterDimension;
+                attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+                attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+                cfg.numAttrs = 2;
+            }
+            BYBYCU_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, cc, pp, part, splits == 1 ? INT32_MAX : split_keys, tile0, tiles, cluster));
+        }
     }
-    BYBYCU_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, c, p, part, splits == 1 ? INT32_MAX : split_keys, row_tiles, cluster));
     return splits > 1 && !cluster ? launch_join(c, p, part, split_keys, 16 * WM, 16, F32, stream) : BYBYCU_OK;
 }
 

@@ -1,13 +1,16 @@
-"""Launches sized for many row tiles."""
+"""Launches of many row tiles or sequences."""
 import pytest
 
 torch = pytest.importorskip("torch")
 
 import kv_helpers  # noqa: E402
 from bybylang_b200 import _lib  # noqa: E402
+from bybylang_b200 import kvcache as kv  # noqa: E402
+from rounding_helpers import scores_off  # noqa: E402
 from test_attention_accuracy import check  # noqa: E402
 
 pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
 
 
 @pytest.mark.parametrize("route", [_lib.ROUTE_AUTO, _lib.ROUTE_GEMV])
@@ -17,6 +20,40 @@ def test_more_row_tiles_than_a_grid_has_rows(route):
     check(bt, route, torch.float32, max_q=32768, max_kv=40000)
     bt = kv_helpers.Batch([(3, 30)], page=16, heads=32, kv_heads=16, dim=256, seed=3)
     check(bt, route, torch.bfloat16, max_q=131072, max_kv=131072)
+
+
+@pytest.mark.parametrize("route", [_lib.ROUTE_AUTO, _lib.ROUTE_GEMV])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_more_sequences_than_a_grid_has_layers(route, dtype):
+    """70000 sequences of one token: each gives its own value."""
+    n, dim = 70000, 8
+    v = torch.randn(n, 1, 1, dim, generator=torch.Generator().manual_seed(4)).to(torch.bfloat16).to(DEV)
+    k, q = torch.ones_like(v), torch.ones(n, 1, dim, dtype=torch.bfloat16, device=DEV)
+    table = torch.arange(n - 1, -1, -1, dtype=torch.int32, device=DEV)[:, None]
+    starts = torch.arange(n + 1, dtype=torch.int32, device=DEV)
+    out = kv.paged_attention(q, k, v, table, starts, torch.ones(n, dtype=torch.int32, device=DEV), max_q=1, max_kv=1, out_dtype=dtype, route=route)
+    torch.cuda.synchronize()
+    assert _lib.device_error() == 0
+    assert torch.equal(out[:, 0], v[:, 0, 0].flip(0).to(dtype))
+
+
+@pytest.mark.parametrize("dim,heads,tokens", [(8, 64, 65537), (136, 32, 131073)])
+def test_prompts_of_more_row_tiles_than_a_grid_has_rows(dim, heads, tokens):
+    """Tokens x heads in tiles of 64 rows, past 65535 of them, under a window: the tensor-core-free
+    routes against each other."""
+    page, n = 64, -(-tokens // 64)
+    g = torch.Generator(device=DEV).manual_seed(7)
+    k, v = (torch.randn(n, 1 if dim > 128 else heads, page, dim, generator=g, device=DEV).to(torch.bfloat16) for _ in range(2))
+    q = torch.randn(tokens, heads, dim, generator=g, device=DEV).to(torch.bfloat16)
+    ints = dict(dtype=torch.int32, device=DEV)
+    batch = k, v, torch.randperm(n, generator=g, device=DEV).to(torch.int32)[None], torch.tensor([0, tokens], **ints), torch.tensor([tokens], **ints)
+    got, want = (kv.paged_attention(q, *batch, max_q=tokens, max_kv=tokens, window=9, out_dtype=torch.float32, route=r)
+                 for r in (_lib.ROUTE_AUTO, _lib.ROUTE_SIMT))
+    torch.cuda.synchronize()
+    assert _lib.device_error() == 0
+    # both exact to fp32: scores_off of each, of values up to 6
+    assert float((got - want).abs().max()) <= 2 * scores_off(1.0) * 6
+    assert torch.isfinite(got).all()
 
 
 @pytest.mark.parametrize("route", [_lib.ROUTE_AUTO, _lib.ROUTE_GEMV, _lib.ROUTE_TC])
