@@ -667,7 +667,7 @@ static int launch(const kvc::Cache& c, const Params& p, const DeviceInfo& info, 
     int64_t splits = active < info.sm_count ? info.sm_count / active : 1;
     const int64_t split_keys64 = std::max<int64_t>(ceil_div(ceil_div(span, splits), kKeys) * kKeys, 4 * kKeys);
     splits = splits == 1 ? 1 : ceil_div(span, split_keys64);
-    const int split_keys = splits == 1 ? INT32_MAX / 2 / kKeys * kKeys : static_cast<int>(split_keys64);
+    const int split_keys = splits == 1 ? INT32_MAX / kKeys * kKeys : static_cast<int>(split_keys64);   // one split: any cache's keys
     if (units * splits > INT32_MAX)
         return set_error(BYBYCU_ERR_SHAPE, "paged_attention: %d sequences, %d kv heads, %d new tokens", c.n_seqs, c.kv_heads, p.max_q);
     Partials part{};

@@ -8,6 +8,8 @@ namespace bybycu {
 namespace kvc {
 
 constexpr int kMaxHeadDim = 256;
+// Positions of a sequence: below 2^31 by more than a kernel looks ahead in 32 bits.
+constexpr int kMaxPositions = INT32_MAX - 8192;
 
 // bybycu_paged_kv by value (kernel parameter).
 struct Cache {
@@ -33,8 +35,8 @@ inline int check_cache(const bybycu_paged_kv* kv, const char* op, Cache* c) {
     if (kv->head_dim < 8 || kv->head_dim > kMaxHeadDim || kv->head_dim % 8)
         return set_error(BYBYCU_ERR_SHAPE, "%s: head dimension %d is not a multiple of 8 up to %d", op, kv->head_dim,
                          kMaxHeadDim);
-    if (static_cast<int64_t>(kv->max_pages) * kv->page_size > INT32_MAX)
-        return set_error(BYBYCU_ERR_SHAPE, "%s: %d pages of %d tokens a sequence exceed 2^31 positions", op,
+    if (static_cast<int64_t>(kv->max_pages) * kv->page_size > kMaxPositions)
+        return set_error(BYBYCU_ERR_SHAPE, "%s: %d pages of %d tokens a sequence exceed 2^31 - 8193 positions", op,
                          kv->max_pages, kv->page_size);
     if (kv->reserved) return set_error(BYBYCU_ERR_ARGS, "%s: reserved fields must be 0", op);
     if (!kv->k || !kv->v || ((!kv->page_table || !kv->kv_lens) && kv->n_seqs > 0) || !kv->q_start)

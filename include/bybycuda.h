@@ -348,7 +348,8 @@ typedef struct bybycu_paged_kv {
     const int32_t* q_start;         /* [n_seqs + 1], not decreasing */
     const int32_t* kv_lens;         /* [n_seqs] */
     int32_t n_pages, page_size, kv_heads, head_dim;   /* head_dim a multiple of 8, at most 256 */
-    int32_t max_pages, n_seqs, n_tokens;              /* n_tokens: rows of q (and k, v) */
+    int32_t max_pages, n_seqs, n_tokens;              /* n_tokens: rows of q (and k, v); max_pages *
+                                                       * page_size at most 2^31 - 8193 */
     int32_t reserved;               /* 0 */
 } bybycu_paged_kv;
 

@@ -61,3 +61,19 @@ def test_a_bound_on_the_new_tokens_may_be_any(route):
     bt = kv_helpers.Batch([(3, 40), (70, 200)], page=16, heads=8, kv_heads=2, dim=64, seed=8)
     for max_q in (73, 1 << 20, 2 ** 31 - 1):
         check(bt, route, torch.bfloat16, max_q=max_q)
+
+
+@pytest.mark.parametrize("route", [_lib.ROUTE_GEMV, _lib.ROUTE_TC, _lib.ROUTE_SIMT])
+def test_the_last_positions_of_the_longest_table(route):
+    """What a window sees does not depend on where it lies: the same cache 2^31 - 12000 positions on."""
+    page, pages = 4096, 524285
+    bt = kv_helpers.Batch([(1, 4000), (40, 4090)], page=page, heads=8, kv_heads=2, dim=64, seed=9)
+    call = dict(max_q=40, window=300, out_dtype=torch.bfloat16, route=route)
+    want = kv.paged_attention(bt.q, *bt.args(), max_kv=4096, **call)
+    table = torch.full((2, pages), -1, dtype=torch.int32, device=DEV)
+    table[:, -1] = bt.table[:, 0]
+    far = bt.kv_lens + (pages - 1) * page
+    got = kv.paged_attention(bt.q, bt.k, bt.v, table, bt.q_start, far, max_kv=pages * page, **call)
+    torch.cuda.synchronize()
+    assert _lib.device_error() == 0
+    assert torch.equal(got, want) and torch.isfinite(got).all() and got.any()

@@ -59,3 +59,11 @@ def test_launches_past_32_bits():
     lib, wide = _lib.load(), dict(q_token_stride=1 << 21, out_token_stride=1 << 21)
     one = dict(kv_heads=1, n_tokens=1 << 16)
     refused(lib.bybycu_paged_attention(cache(**one), attention(q_heads=1 << 15, max_q=1 << 16, **wide), None), _lib.ERR_SHAPE, "2^31 rows")
+
+
+@no_device
+@pytest.mark.parametrize("max_pages,page_size", [(524286, 4096), (1, 2 ** 31 - 8192), (2 ** 31 - 1, 1)])
+def test_tables_close_to_2_31_positions(max_pages, page_size):
+    kw = dict(max_pages=max_pages, page_size=page_size, table_stride=max_pages, head_stride=page_size * 64, page_stride=4 * page_size * 64)
+    refused(_lib.load().bybycu_paged_attention(cache(**kw), attention(), None), _lib.ERR_SHAPE, "2^31 - 8193")
+    refused(_lib.load().bybycu_rope_append(cache(**kw), rope(), None), _lib.ERR_SHAPE, "2^31 - 8193")
