@@ -251,7 +251,8 @@ def copy_pages(k_cache, v_cache, pairs, *, stream=None) -> None:
 def beam_select(logits, scores, keep: int, *, stream=None):
     """The `keep` best continuations of each group: logits [groups * beams, vocab] float32 or
     bfloat16, scores float32 [groups, beams] the beams' log-probabilities so far.  Returns (scores
-    float32, beams int32, tokens int32), each [groups, keep], best first."""
+    float32, beams int32, tokens int32), each [groups, keep], best first; equal scores by the lower
+    beam, within a beam by the larger logit, then the lower token."""
     import torch
     if logits.dim() != 2 or scores.dim() != 2 or logits.shape[0] != scores.numel():
         _refuse(_lib.ERR_SHAPE, f"beam_select: logits {tuple(logits.shape)} for scores {tuple(scores.shape)}")

@@ -413,11 +413,14 @@ BYBYCU_API int bybycu_copy_pages(void* k, void* v, int n_layers, int64_t layer_s
                                  int64_t page_bytes, int n_pages, const int32_t* pairs, int n_pairs, void* stream);
 
 /* Beam search's selection: of the groups' beams * vocab continuations each the `keep` best by
- * scores[g][b] + logits[row][t] - logsumexp(logits[row]), row = g * beams + b, best first, equal
- * scores by the lower b, then the lower t.  A NaN sum (a row with no finite logit, with NaN or
- * with +inf) counts as -inf.  logits F32 or BF16 [groups * beams, vocab], rows row_stride elements
- * apart; scores fp32 [groups, beams]; the outputs [groups, keep].  1 <= keep <= 64, at most
- * beams * vocab; beams <= 64, vocab <= 2^20, at most 65535 rows. */
+ * scores[g][b] + ((logits[row][t] - m) - log(sum_t exp(logits[row][t] - m))), m the row's largest
+ * logit, row = g * beams + b, best first.  Between beams the fp32 scores decide, equal ones by the
+ * lower b; within a beam the logits do, equal ones by the lower t: that is the order of the exact
+ * scores, also where they round alike.  A beam that cannot go on (a row with no finite logit, with
+ * NaN or with +inf, or a score of -inf or NaN) gives -inf, its tokens in their own order.  logits
+ * F32 or BF16 [groups * beams, vocab], rows row_stride elements apart; scores fp32 [groups, beams];
+ * the outputs [groups, keep].  1 <= keep <= 64, at most beams * vocab; beams <= 64, vocab <= 2^20,
+ * at most 65535 rows. */
 BYBYCU_API int bybycu_beam_select(const void* logits, int logits_dtype, int64_t row_stride, const float* scores,
                                   int groups, int beams, int vocab, int keep, float* out_scores,
                                   int32_t* out_beams, int32_t* out_tokens, void* stream);

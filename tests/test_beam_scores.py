@@ -75,3 +75,31 @@ def test_offset_rows_in_bf16():
     g = torch.Generator().manual_seed(1)
     x = 2 * torch.randn(8, 32768, generator=g) + torch.tensor([0.0, 100, -100, 200, -200, 30, 500, -500])[:, None]
     against64(x.to(torch.bfloat16).to(DEV), (-4 * torch.rand(2, 4, generator=g)).to(DEV), 16)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("prior", [-1e9, -1e20])
+def test_priors_that_swallow_the_logits(prior, dtype):
+    """All of a beam's continuations round to its sentinel: they keep the order of their logits,
+    equal logits that of their tokens, and a beam's order is the lower beam's first."""
+    g = torch.Generator().manual_seed(11)
+    x = (torch.randn(3, 5000, generator=g) * 2).to(dtype)
+    x[1, 100] = x[1, 4000] = x[1].max() + 1
+    s = torch.tensor([[prior, prior, 2 * prior]])
+    score, beam, token = kv.beam_select(x.to(DEV), s.to(DEV), 12)
+    assert beam.tolist() == [[0] * 12] and (score == prior).all()
+    assert token[0].tolist() == torch.sort(x[0].float(), descending=True, stable=True).indices[:12].tolist()
+    score, beam, token = kv.beam_select(x[1:].contiguous().to(DEV), torch.tensor([[prior, -1.0]], device=DEV), 64)
+    assert (beam == 1).all()
+    score, beam, token = kv.beam_select(x[1:2].to(DEV), torch.tensor([[prior]], device=DEV), 5)
+    assert token[0].tolist() == torch.sort(x[1].float(), descending=True, stable=True).indices[:5].tolist() and token[0, :2].tolist() == [100, 4000]
+
+
+def test_beams_whose_scores_round_alike():
+    """Two beams with the same logits: at equal scores the lower beam comes first, each with its
+    continuations in the order of their logits."""
+    x = torch.full((2, 300), -50.0)
+    x[:, [250, 17, 40]] = torch.tensor([2.0, 2.0 + 2.0 ** -22, 1.0])
+    score, beam, token = kv.beam_select(x.to(DEV), torch.full((1, 2), -1000.0, device=DEV), 6)
+    got = list(zip(beam[0].tolist(), token[0].tolist()))
+    assert got == [(0, 17), (0, 250), (1, 17), (1, 250), (0, 40), (1, 40)]
