@@ -23,8 +23,10 @@ A batch is three int32 device tensors: ``page_table`` [sequences, pages], ``q_st
 """
 from __future__ import annotations
 
+import array
 import ctypes as C
 import heapq
+import itertools
 import math
 import struct
 
@@ -214,6 +216,28 @@ def paged_attention(q, k_cache, v_cache, page_table, q_start, kv_lens, *, max_q:
     return out
 
 
+def _pairs(pairs):
+    """The pairs of a copy as contiguous int32 [n, 2] on the host."""
+    import torch
+    if isinstance(pairs, (list, tuple)):
+        try:
+            if not all(len(p) == 2 for p in pairs):
+                _refuse(_lib.ERR_SHAPE, f"copy_pages: pairs are {pairs!r:.60}, not [n, 2]")
+            flat = array.array("i", itertools.chain.from_iterable(pairs))
+        except (TypeError, OverflowError):
+            _refuse(_lib.ERR_ARGS, "copy_pages: pairs must be whole numbers that fit 32 bits, two each")
+        return torch.frombuffer(flat, dtype=torch.int32).view(-1, 2) if flat else torch.empty(0, 2, dtype=torch.int32)
+    p = torch.as_tensor(pairs, device="cpu")
+    if (p.dim() != 2 or p.shape[1] != 2) and (p.numel() or p.dim() == 0):
+        _refuse(_lib.ERR_SHAPE, f"copy_pages: pairs are {tuple(p.shape)}, not [n, 2]")
+    if p.dtype != torch.int32 and p.numel():
+        wide = p.to(torch.int64)
+        if p.dtype.is_floating_point or p.dtype.is_complex or p.dtype == torch.bool or wide.min() < -(1 << 31) or wide.max() >= 1 << 31:
+            _refuse(_lib.ERR_ARGS, "copy_pages: pairs must be whole numbers that fit 32 bits, two each")
+        p = wide
+    return p.to(torch.int32).contiguous()
+
+
 def copy_pages(k_cache, v_cache, pairs, *, stream=None) -> None:
     """Page dst becomes page src for each (src, dst) of `pairs` (host: int32 [n, 2] tensor or
     array, or a list), in every layer of caches [layers, pages, ...] (bf16 or any other type; 4-D
@@ -239,10 +263,8 @@ def copy_pages(k_cache, v_cache, pairs, *, stream=None) -> None:
             run *= n
     if n_pages == 1:
         page_stride = dense
-    p = torch.as_tensor(pairs, dtype=torch.int32, device="cpu").contiguous()
+    p = _pairs(pairs)
     n = p.shape[0] if p.numel() else 0
-    if n and (p.dim() != 2 or p.shape[1] != 2):
-        _refuse(_lib.ERR_SHAPE, f"copy_pages: pairs are {tuple(p.shape)}, not [n, 2]")
     esz = k_cache.element_size()
     check(_call("bybycu_copy_pages")(k_cache.data_ptr(), 0 if v_cache is None else v_cache.data_ptr(), layers, layer_stride * esz,
                                      page_stride * esz, dense * esz, n_pages, p.data_ptr(), n, _stream("copy_pages", dev, stream)))
