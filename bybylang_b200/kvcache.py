@@ -219,6 +219,8 @@ def paged_attention(q, k_cache, v_cache, page_table, q_start, kv_lens, *, max_q:
 def _pairs(pairs):
     """The pairs of a copy as contiguous int32 [n, 2] on the host."""
     import torch
+    if isinstance(pairs, torch.Tensor) and pairs.dtype == torch.int32 and pairs.is_cpu and pairs.dim() == 2 and pairs.shape[1] == 2:
+        return pairs.contiguous()
     if isinstance(pairs, (list, tuple)):
         try:
             if not all(len(p) == 2 for p in pairs):
