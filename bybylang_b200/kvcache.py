@@ -393,6 +393,10 @@ class PagePool:
 
     def reorder(self, seqs: list[int], parents: list[int]) -> list[int]:
         """Beam search's step: sequence i of the result continues seqs[parents[i]]; the old ones are freed."""
+        for q in seqs:
+            self._seq(q)
+        if len(set(seqs)) != len(seqs) or not all(0 <= p < len(seqs) for p in parents):
+            _refuse(_lib.ERR_ARGS, f"PagePool: parents {parents} of {len(seqs)} different sequences")
         new = [self.fork(seqs[p]) for p in parents]
         for s in seqs:
             self.free(s)

@@ -31,3 +31,27 @@ def test_pairs(pairs, want):
 def test_pairs_of_another_shape(pairs):
     with pytest.raises(_lib.BybyCudaError, match="not \\[n, 2\\]"):
         kv._pairs(pairs)
+
+
+@pytest.mark.parametrize("seqs,parents", [("ab", [0, 2]), ("ab", [0, -1]), ("ab", [1, 0, 7]), ("aa", [0, 1]), ("a?", [0, 0]), ("a?", [0, 1])])
+def test_a_refused_reorder_changes_nothing(seqs, parents):
+    pool = kv.PagePool(8, 4)
+    a, b = pool.new(), pool.new()
+    pool.extend(a, 6)
+    pool.extend(b, 3)
+    ids = [{"a": a, "b": b, "?": 99}[x] for x in seqs]
+    before = (list(pool._refs), pool.free_pages, pool.pages(a), pool.pages(b), pool.length(a), pool.length(b), sorted(pool._seqs))
+    with pytest.raises(_lib.BybyCudaError):
+        pool.reorder(ids, parents)
+    assert before == (list(pool._refs), pool.free_pages, pool.pages(a), pool.pages(b), pool.length(a), pool.length(b), sorted(pool._seqs))
+
+
+def test_reorder_to_more_and_fewer():
+    pool = kv.PagePool(8, 4)
+    a, b = pool.new(), pool.new()
+    pool.extend(a, 6)
+    pool.extend(b, 3)
+    c, d, e = pool.reorder([a, b], [1, 1, 0])
+    assert [pool.length(s) for s in (c, d, e)] == [3, 3, 6] and pool.pages(c) == pool.pages(d)
+    f, = pool.reorder([c, d, e], [2])
+    assert pool.length(f) == 6 and pool.free_pages == 6
