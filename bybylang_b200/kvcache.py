@@ -57,6 +57,13 @@ def _refuse(code: int, message: str):
     raise BybyCudaError(code, message)
 
 
+def _pack(op: str, pack, *fields) -> bytes:
+    try:
+        return pack(*fields)
+    except (struct.error, OverflowError) as e:
+        _refuse(_lib.ERR_ARGS, f"{op}: an argument does not fit its field ({e})")
+
+
 def _stream(op: str, device: int, stream) -> int:
     """The raw stream of a call on `device`, which has to be the current one and the stream's (the
     default stream has one handle on every device)."""
@@ -178,7 +185,7 @@ def rope_append(q, k, v, k_cache, v_cache, page_table, q_start, kv_lens, turns, 
     else:
         os_ = _heads("rope_append", "q_out", q_out, T, hq, dim, dev, torch.bfloat16)
     pairs = turns.numel()
-    args = _ROPE(q.data_ptr(), k.data_ptr(), v.data_ptr(), q_out.data_ptr(), *qs, *ks, *vs, *os_,
+    args = _pack("rope_append", _ROPE, q.data_ptr(), k.data_ptr(), v.data_ptr(), q_out.data_ptr(), *qs, *ks, *vs, *os_,
                  _vector("rope_append", "turns", turns, pairs, torch.float64, dev),
                  _vector("rope_append", "positions", positions, T, torch.int32, dev), _dtype_code(q), hq, pairs,
                  _LAYOUTS[layout], magnitude, 0)
@@ -209,7 +216,7 @@ def paged_attention(q, k_cache, v_cache, page_table, q_start, kv_lens, *, max_q:
         os_ = hq * dim, dim
     else:
         os_ = _heads("paged_attention", "out", out, T, hq, dim, dev, out_dtype)
-    args = _ATTENTION(q.data_ptr(), out.data_ptr(), *qs, *os_, _vector("paged_attention", "slopes", slopes, hq, torch.float32, dev),
+    args = _pack("paged_attention", _ATTENTION, q.data_ptr(), out.data_ptr(), *qs, *os_, _vector("paged_attention", "slopes", slopes, hq, torch.float32, dev),
                       _vector("paged_attention", "prefix_lens", prefix_lens, n_seqs, torch.int32, dev), _dtype_code(out), hq,
                       max_q, max_kv, window, route, dim ** -0.5 if scale is None else scale, softcap)
     check(_call("bybycu_paged_attention")(kv, args, raw))
@@ -286,6 +293,8 @@ def beam_select(logits, scores, keep: int, *, stream=None):
     if scores.dtype != torch.float32 or not scores.is_contiguous() or dev < 0 or scores.get_device() != dev or (vocab > 1 and one != 1):
         _refuse(_lib.ERR_ARGS, "beam_select: scores must be contiguous float32, the rows of logits dense, both on the device")
     groups, beams = scores.shape
+    if not 1 <= keep <= 64 or keep > beams * vocab:
+        _refuse(_lib.ERR_SHAPE, f"beam_select: groups={groups} beams={beams} vocab={vocab} keep={keep}")
     raw = _stream("beam_select", dev, stream)
     best = _output((groups, keep), torch.float32, logits.device, stream)
     which = _output((2, groups, keep), torch.int32, logits.device, stream)

@@ -55,3 +55,23 @@ def test_reorder_to_more_and_fewer():
     assert [pool.length(s) for s in (c, d, e)] == [3, 3, 6] and pool.pages(c) == pool.pages(d)
     f, = pool.reorder([c, d, e], [2])
     assert pool.length(f) == 6 and pool.free_pages == 6
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kw", [dict(max_q=1 << 31), dict(max_kv=1 << 40), dict(window=-(1 << 40)), dict(scale=1e300), dict(softcap=1e300), dict(route=1 << 33),
+                                dict(max_q=2.5)], ids=str)
+def test_numbers_that_do_not_fit(kw):
+    from kv_helpers import Batch
+    bt = Batch([(1, 20)], page=16, heads=4, kv_heads=2, dim=64, seed=1)
+    with pytest.raises(_lib.BybyCudaError, match="paged_attention"):
+        kv.paged_attention(bt.q, *bt.args(), **{**dict(max_q=1, max_kv=20), **kw})
+    x = torch.zeros(1, 8, 64, device=bt.q.device)
+    with pytest.raises(_lib.BybyCudaError, match="rope_append"):
+        kv.rope_append(x[:, :4], x[:, 4:6], x[:, 6:], *bt.args(), kv.rope_frequencies(64), magnitude=1e300)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("keep", [-1, 0, 65, 1 << 40])
+def test_a_keep_out_of_range(keep):
+    with pytest.raises(_lib.BybyCudaError, match="keep="):
+        kv.beam_select(torch.zeros(2, 100, device="cuda:0"), torch.zeros(1, 2, device="cuda:0"), keep)
