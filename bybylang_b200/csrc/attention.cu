@@ -149,7 +149,7 @@ extern "C" int bybycu_paged_attention(const bybycu_paged_kv* kv, const bybycu_at
     const bool tc = attn::tc_attention_supports(c, p, f32);
     if (a->route == BYBYCU_ROUTE_TC && !tc)
         return set_error(BYBYCU_ERR_SHAPE, "paged_attention: the tensor-core route needs bf16 output, head dimension <= 128, at most "
-                                           "128 heads a group and pages of 8, 16, 32, 64 or a multiple of 128 tokens");
+                                           "128 heads a group, pages of 8, 16, 32, 64 or a multiple of 128 tokens and a token stride of q");
     // A tensor-core tile costs its 128 rows however many there are, the GEMV's warps 16 each: 8
     // sequences of 4096 keys, 8 kv heads of 128, at 16, 32, 64 and 128 rows 51, 64, 88, 153 us on
     // the GEMV and 43, 46, 51, 61 on the tensor cores; heads of 64 33, 41, 53, 93 and 37, 39, 43,

@@ -623,7 +623,7 @@ static int encode_map(CUtensorMap* map, const void* base, int rank, const int64_
         d[i] = static_cast<cuuint64_t>(dims[i]);
         bx[i] = static_cast<cuuint32_t>(box[i]);
         es[i] = 1;
-        if (i) st[i - 1] = static_cast<cuuint64_t>(std::max<int64_t>(strides[i] * 2, 16));   // a stride of one element is never used
+        if (i) st[i - 1] = static_cast<cuuint64_t>(std::max<int64_t>(strides[i] * 2, 16));   // 0 only along a dimension of 1, never stepped
     }
     const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, static_cast<cuuint32_t>(rank), const_cast<void*>(base), d, st, bx, es,
                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -689,10 +689,11 @@ static int launch(const kvc::Cache& c, const Params& p, const DeviceInfo& info, 
 }  // namespace tcore
 
 // Head dimensions up to 128, groups up to 128 heads, pages that tile a block of 128 keys (or are
-// tiled by it) in whole swizzle atoms of 8 slots.
+// tiled by it) in whole swizzle atoms of 8 slots, and queries that step from token to token (a tensor
+// map's strides are 16 bytes at least).
 static bool tc_attention_supports(const kvc::Cache& c, const Params& p, bool f32) {
     const bool pages = c.page_size % 8 == 0 && (tcore::kKeys % c.page_size == 0 || c.page_size % tcore::kKeys == 0);
-    return !f32 && c.head_dim <= 128 && p.group <= tcore::kRows && pages;
+    return !f32 && c.head_dim <= 128 && p.group <= tcore::kRows && pages && (p.q_token > 0 || c.n_tokens == 1);
 }
 
 static int launch_tc_attention(const kvc::Cache& c, const Params& p, bool mod, cudaStream_t stream) {

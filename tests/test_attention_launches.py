@@ -77,3 +77,21 @@ def test_the_last_positions_of_the_longest_table(route):
     torch.cuda.synchronize()
     assert _lib.device_error() == 0
     assert torch.equal(got, want) and torch.isfinite(got).all() and got.any()
+
+
+@pytest.mark.parametrize("route", [_lib.ROUTE_AUTO, _lib.ROUTE_GEMV, _lib.ROUTE_SIMT])
+def test_one_query_for_every_token(route):
+    """q expanded over the tokens (stride 0): the tensor-core route cannot step by it and is not taken."""
+    bt = kv_helpers.Batch([(70, 200), (3, 40)], page=16, heads=8, kv_heads=2, dim=64, seed=10)
+    bt.q = bt.q[:1].expand(bt.tokens, 8, 64)
+    assert bt.q.stride(0) == 0
+    check(bt, route, torch.bfloat16)
+
+
+def test_one_query_for_every_token_is_refused_on_the_tensor_cores():
+    bt = kv_helpers.Batch([(70, 200)], page=16, heads=8, kv_heads=2, dim=64, seed=10)
+    with pytest.raises(_lib.BybyCudaError, match="token stride of q"):
+        kv.paged_attention(bt.q[:1].expand(70, 8, 64), *bt.args(), max_q=70, max_kv=200, route=_lib.ROUTE_TC)
+    one = kv_helpers.Batch([(1, 200)], page=16, heads=8, kv_heads=2, dim=64, seed=10)     # a single token needs none
+    one.q = one.q.as_strided((1, 8, 64), (0, 64, 1))
+    check(one, _lib.ROUTE_TC, torch.bfloat16)
