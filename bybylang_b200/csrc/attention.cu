@@ -153,7 +153,10 @@ extern "C" int bybycu_paged_attention(const bybycu_paged_kv* kv, const bybycu_at
     // A tensor-core tile costs its 128 rows however many there are, the GEMV's warps 16 each: 8
     // sequences of 4096 keys, 8 kv heads of 128, at 16, 32, 64 and 128 rows 51, 64, 88, 153 us on
     // the GEMV and 43, 46, 51, 61 on the tensor cores; heads of 64 33, 41, 53, 93 and 37, 39, 43,
-    // 53; one sequence of 2048 15, 17, 21, 23 and 19, 19, 20, 23.
+    // 53; one sequence of 2048 15, 17, 21, 23 and 19, 19, 20, 23.  From 33 rows on the tensor cores
+    // are ahead in all three.  Up to 32 the rule keeps the GEMV, which one short sequence is faster
+    // on; a batch of 17 to 32 rows a kv head is up to 28% slower by it (the number of tiles, which
+    // would tell the two apart, is not part of the rule).
     if (a->route == BYBYCU_ROUTE_TC || (a->route == BYBYCU_ROUTE_AUTO && tc && static_cast<int64_t>(max_q) * p.group > 32))
         return attn::launch_tc_attention(c, p, mod, s);
     return attn::launch_gemv(c, p, f32, s);

@@ -13,8 +13,9 @@
 // exponentials: at 128 dimensions a block's two products take the tensor core about as long
 // (2 * 128^3 multiplies at 4096 a cycle) as its 128^2 exponentials take the SM's special-function
 // units (16 a cycle), so neither may wait for the other.
-//   Measured: 2 sequences of 4096 tokens, 32 heads of 128, 281 us (980 TFLOP/s); with 8 kv heads
-// 274 us; heads of 64 at half of that rate (the exponentials are the same).  A pair of blocks takes
+//   Measured: 2 sequences of 4096 tokens, 32 heads of 128, 281 us (980 TFLOP/s) alone, 323 us where
+// call follows call and the clocks give way; with 8 kv heads 274 us; heads of 64 at half of that
+// rate (the exponentials are the same).  A pair of blocks takes
 // some 3300 cycles where its MMAs alone are 2048: a tile's softmax (1700, issue and latency of four
 // warps on a scheduler) and its own P V and S (1350) follow one another, and only the other tile's
 // run beside them.
@@ -27,6 +28,9 @@
 //     these steps outside the common range are zeroed in shared memory (0 * NaN would be NaN).
 //   * bf16 output only: the tensor core truncates when it accumulates, and over thousands of keys
 //     that costs an fp32 output two digits.
+//   * Fewer bits than fp32, for a bf16 output: probabilities in bf16 (16 bits would take half as much
+//     tensor work again), the cubic of ex2_fma, the truncation, a cap up to 256 in its
+//     plain form.  2.0e-3 of the output's norm together, of which its own rounding is 1.7e-3.
 //
 // Every wait is bounded: on a timeout the kernel records the error, drains its copies and MMAs,
 // frees its tensor memory and returns.

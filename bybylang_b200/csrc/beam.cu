@@ -136,9 +136,10 @@ __device__ __forceinline__ void warp_merge(const uint64_t* lists, int n_lists, i
 // not below the smallest of these.  After 2, 4, 8, 16 and 32 chunks the same with the r-th best
 // candidates, so that for logits in no particular order some 2 * keep / c elements of the c-th
 // chunks become candidates.  A warp that has more than kSoft cuts them down to its best keep.
-// 256 rows of 128256 bf16 (66 MB) take 42 us with the second kernel, 1.6 TB/s: bound by the
-// instructions a logit (block-wide bounds met at a barrier every 2048 logits took 61 us, a warp's
-// bound from its own first 256 logits 80 us).
+// 256 rows of 128256 bf16 (66 MB) take 43 us with the second kernel, 1.5 TB/s: bound by the 20
+// instructions a logit, of which the conversion, maximum, sum and comparison need about 8 (block-wide
+// bounds met at a barrier every 2048 logits took 61 us, a warp's bound from its own first 256 logits
+// 80 us).
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kThreads, 4) beam_scan_kernel(const Params p) {
     __shared__ uint64_t s_cand[kWarps * kCand];

@@ -166,7 +166,8 @@ def rope_append(q, k, v, k_cache, v_cache, page_table, q_start, kv_lens, turns, 
     projection, float32 or bfloat16.  turns: fp64 [pairs], the turns per position of each pair
     (``rope_frequencies``); 2 * pairs dimensions turn, the rest pass.  layout "half" pairs (i, i +
     pairs), "interleaved" (2i, 2i + 1).  positions (int32 [tokens]) turns by other positions than
-    those in the cache.  A token at a negative position is padding: its queries come back zero."""
+    those in the cache.  A token at a negative position is padding: its queries come back zero.  Rows that belong to
+    no sequence (before q_start[0], from q_start[-1] on) are not written: whatever the output held."""
     import torch
     if q.dim() != 3:
         _refuse(_lib.ERR_SHAPE, f"rope_append: q is {tuple(q.shape)}, not [tokens, heads, dim]")
@@ -203,7 +204,8 @@ def paged_attention(q, k_cache, v_cache, page_table, q_start, kv_lens, *, max_q:
     tanh(score / softcap); slopes (float32 [heads]) subtracts slope * distance; window > 0 hides
     keys `window` or more positions back; prefix_lens (int32 [sequences]) lets every row see the
     first prefix_lens[b] keys.  The output is q's shape in out_dtype (bfloat16 by default, or
-    float32); rows that see nothing are zero."""
+    float32), its vectors apart from one another; rows that see nothing are zero, rows that belong to
+    no sequence (before q_start[0], from q_start[-1] on) are not written: whatever the output held."""
     import torch
     if q.dim() != 3:
         _refuse(_lib.ERR_SHAPE, f"paged_attention: q is {tuple(q.shape)}, not [tokens, heads, dim]")

@@ -383,15 +383,26 @@ BYBYCU_API int bybycu_rope_append(const bybycu_paged_kv* kv, const bybycu_rope* 
  * not used, whatever they hold.  A key that a row does not see does not reach it; a value that is
  * not finite does where another row of the same launch tile sees it (0 * NaN).
  *   max_q, max_kv bound the new tokens and the cache length of every sequence (the launch is sized
- *   by them); a sequence beyond either records device error 10 and its rows beyond are not
- *   computed.
+ *   by them, max_q no larger than n_tokens); a sequence beyond either records device error 10 and
+ *   its rows beyond are not computed.  n_tokens x heads of a group stays below 2^31.
+ *   q may be one token for all (token stride 0); the vectors of `out` may not overlap.
  *   route AUTO: TC (tcgen05) for more than 32 query rows (new tokens x heads of a group) a kv head
  *   where it applies - bf16 output, head dimension up to 128, groups up to 128 heads, pages of 8,
- *   16, 32, 64 or a multiple of 128 tokens - else GEMV (warp-level MMAs, the cache split over the
- *   grid), which runs every shape.  SIMT: one warp a row, fp32 FMAs, every shape; only when asked
- *   for.  An explicit TC that does not apply returns BYBYCU_ERR_SHAPE.
- * Scores, softmax statistics and sums are fp32.  The probabilities enter the product with V as
- * bf16 for a bf16 output, as three bf16 terms (24 bits) for an fp32 output (SIMT: fp32). */
+ *   16, 32, 64 or a multiple of 128 tokens, a token stride of q - else GEMV (warp-level MMAs, the
+ *   cache split over the grid), which runs every shape, in several launches past 65535 row tiles x
+ *   kv heads or sequences (at most 65535 kv heads).  SIMT: one warp a row, fp32 FMAs, every shape;
+ *   only when asked for.  An explicit TC that does not apply returns BYBYCU_ERR_SHAPE.
+ * Scores, softmax statistics and sums are fp32 on every route.  What has fewer bits than an fp32
+ * computation rounded once at the end:
+ *   - the probabilities enter the product with V as bf16 for a bf16 output (TC, GEMV), as three
+ *     bf16 terms (24 bits) for an fp32 output (GEMV); SIMT has them in fp32;
+ *   - the tensor core truncates as it accumulates: for a bf16 output over the whole cache, 3e-6
+ *     of a sum over 131071 keys; an fp32 output adds each chunk with a rounding;
+ *   - TC takes 3 of 16 exponentials of unmasked keys with a cubic, good to 7.5e-5;
+ *   - softcap up to 256 and a bf16 output: the capped score is good to 1e-7 of the cap; any other
+ *     to a few 2^-24 of the score.
+ * A bf16 output of normal values is so 2.0e-3 (TC) to 2.3e-3 (GEMV) of its norm from the exact one,
+ * where its own rounding alone is 1.7e-3; an fp32 output 3e-7. */
 typedef struct bybycu_attention {
     const void* q;                  /* bf16 [n_tokens, q_heads, head_dim] */
     void* out;                      /* out_dtype, same shape */
